@@ -43,6 +43,24 @@ class ProfileRow(C.Structure):
     ]
 
 
+class NormArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "h", "x_out", "u", "post_weight", "post_bias", "pre_weight", "pre_bias", "gate",
+                                          "slots", "weights")] + [
+        ("rows", C.c_int64),
+        ("h_rows", C.c_int64),
+        ("gate_rows", C.c_int64),
+        ("width", C.c_int),
+        ("k", C.c_int),
+        ("x_dtype", C.c_int),
+        ("h_dtype", C.c_int),
+        ("gate_dtype", C.c_int),
+        ("gate_act", C.c_int),
+        ("layer", C.c_int),
+        ("scale", C.c_float),
+        ("eps", C.c_float),
+    ]
+
+
 class Param(C.Structure):
     _fields_ = [
         ("name", C.c_char_p),
@@ -99,6 +117,12 @@ SIGNATURES = {
     "fd_detect_graph_launch": (C.c_int, [vp, vp]),
     "fd_detect_graph_destroy": (None, [vp]),
     "fd_detector_keep_tensors": (C.c_int, [vp, C.c_int]),
+    "fd_expert_route_workspace": (C.c_int64, [C.c_int64, C.c_int]),
+    "fd_expert_route": (C.c_int, [vp, C.c_int, C.c_int64, C.c_int, C.c_int, vp, C.c_int, vp, vp, vp, vp, vp, vp, C.c_int64, vp]),
+    "fd_expert_linear": (C.c_int, [vp, C.c_int, C.c_int64, C.c_int, vp, C.c_int, C.c_int, vp, vp, C.c_int64, vp, C.c_int, C.c_int,
+                                   vp, vp]),
+    "fd_expert_combine": (C.c_int, [vp, C.c_int, C.c_int64, C.c_int, vp, vp, C.c_int64, C.c_int, vp, vp]),
+    "fd_residual_norm": (C.c_int, [C.POINTER(NormArgs), vp]),
     "fd_detector_tensor": (C.c_int, [vp, C.c_char_p, vp, C.c_int64, C.POINTER(C.c_int64), vp]),
 }
 

@@ -1,0 +1,261 @@
+// Norms around a residual block, with the block's gate, residual scale and (for a block of experts) the weighted
+// sum of a row's expert outputs; and that sum on its own.
+//
+//   h[t]  = sum_j weights[t,j] * y[slots[t,j]]            (expert blocks; otherwise h is read as it is)
+//   x'[t] = x[t] + scale * act(gate) * norm(h[t])
+//   u[t]  = norm(x'[t])
+//   norm(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps) * weight + bias,  mean = 0 for the RMS form
+//
+// Bound by memory: a row is read once, held in registers as float32 through all of this, and written once.  Means and
+// squares are summed in float32 over the registers (two passes, no E[v^2] - mean^2), so the only rounding to the
+// tensors' type is the one at the store; u is computed from the unrounded x'.
+#include "fd_elem.h"
+
+namespace fd {
+
+struct NormArgs {
+    const void *x, *h, *gate;
+    const float *post_weight, *post_bias, *pre_weight, *pre_bias, *weights;
+    const int32_t* slots;
+    void *x_out, *u;
+    int64_t rows, h_rows;
+    int width, k, rows_per_gate, gate_f32, gate_act, layer;
+    float scale, eps;
+};
+
+__device__ __forceinline__ float gate_value(float g, int act) {
+    if (act == FD_GATE_SIGMOID) return 1.f / (1.f + expf(-g));
+    if (act == FD_GATE_TANH) return tanhf(g);
+    return g;
+}
+
+// Sum over the G lanes that share a row; every lane gets it.  G = 256 goes through LDS, alternating between two sets
+// of words so that one barrier a sum is enough.
+template <int G>
+__device__ __forceinline__ float row_sum(float v, float (*part)[4], int& turn) {
+#pragma unroll
+    for (int d = (G < 64 ? G : 64) / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+    if (G == 256) {
+        if ((threadIdx.x & 63) == 0) part[turn][threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = (part[turn][0] + part[turn][1]) + (part[turn][2] + part[turn][3]);
+        turn ^= 1;
+    }
+    return v;
+}
+
+template <int G, int NC>
+__device__ __forceinline__ void normalise(float (&v)[NC][8], const float* weight, const float* bias, const NormArgs& a, int lane,
+                                          float (*part)[4], int& turn) {
+    if (a.layer) {
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[c][i];
+        const float mean = row_sum<G>(s, part, turn) / (float)a.width;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if ((c * G + lane) * 8 + i < a.width) v[c][i] -= mean;
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v[c][i] * v[c][i];
+    const float r = rsqrtf(row_sum<G>(s, part, turn) / (float)a.width + a.eps);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int col = (c * G + lane) * 8;
+        float w[8], b[8];
+        load8(weight + col, a.width - col, w);
+        if (bias) load8(bias + col, a.width - col, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] = v[c][i] * r * w[i] + (bias ? b[i] : 0.f);
+    }
+}
+
+// G lanes hold a row, NC pieces of 8 elements each: element (c * G + lane) * 8 + i.
+template <typename TX, typename TH, int G, int NC>
+__global__ __launch_bounds__(256) void residual_norm_kernel(NormArgs a) {
+    __shared__ float part[2][4];
+    int turn = 0;
+    const int lane = threadIdx.x % G;
+    const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    if (row >= a.rows) return;                       // a whole group of G lanes: G = 256 never leaves early
+    float x[NC][8];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int col = (c * G + lane) * 8;
+        load8((const TX*)a.x + row * a.width + col, a.width - col, x[c]);
+    }
+    if (a.h) {
+        float h[NC][8];
+        if (a.slots) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[c][i] = 0.f;
+            for (int j = 0; j < a.k; ++j) {
+                const int32_t s = a.slots[row * a.k + j];
+                if (s < 0 || s >= a.h_rows) continue;
+                const float w = a.weights[row * a.k + j];
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const int col = (c * G + lane) * 8;
+                    float y[8];
+                    load8((const TH*)a.h + (int64_t)s * a.width + col, a.width - col, y);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) h[c][i] += w * y[i];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int col = (c * G + lane) * 8;
+                load8((const TH*)a.h + row * a.width + col, a.width - col, h[c]);
+            }
+        }
+        if (a.post_weight) normalise<G, NC>(h, a.post_weight, a.post_bias, a, lane, part, turn);
+        const int64_t gate_row = a.gate ? (row / a.rows_per_gate) * a.width : 0;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * G + lane) * 8;
+            if (a.gate) {
+                float g[8];
+                if (a.gate_f32) load8((const float*)a.gate + gate_row + col, a.width - col, g);
+                else load8((const TH*)a.gate + gate_row + col, a.width - col, g);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[c][i] *= gate_value(g[i], a.gate_act);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (col + i < a.width) x[c][i] += a.scale * h[c][i];
+            store8((TX*)a.x_out + row * a.width + col, a.width - col, x[c]);
+        }
+    }
+    if (a.pre_weight) {
+        normalise<G, NC>(x, a.pre_weight, a.pre_bias, a, lane, part, turn);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * G + lane) * 8;
+            store8((TH*)a.u + row * a.width + col, a.width - col, x[c]);
+        }
+    }
+}
+
+template <typename TX, typename TH>
+static int launch_residual_norm(const NormArgs& a, hipStream_t stream) {
+    // Lanes per row: the fewest that hold it in at most 4 pieces a lane.  Wide rows, and rows of more than 512
+    // elements when there are too few to give every CU eight waves, take a whole workgroup.
+    const bool few = a.rows < 2048 && a.width > 512;
+#define FD_NORM(G, NC)                                                                                                \
+    do {                                                                                                              \
+        const int64_t blocks = (a.rows + 256 / G - 1) / (256 / G);                                                    \
+        hipLaunchKernelGGL((residual_norm_kernel<TX, TH, G, NC>), dim3((unsigned)blocks), dim3(256), 0, stream, a);   \
+    } while (0)
+    if (a.width <= 128) FD_NORM(16, 1);
+    else if (a.width <= 512) FD_NORM(64, 1);
+    else if (few && a.width <= 2048) FD_NORM(256, 1);
+    else if (a.width <= 1024) FD_NORM(64, 2);
+    else if (a.width <= 2048) FD_NORM(64, 4);
+    else if (a.width <= 4096) FD_NORM(256, 2);
+    else if (a.width <= 8192) FD_NORM(256, 4);
+    else FD_NORM(256, 8);
+#undef FD_NORM
+    FD_LAUNCH_CHECK();
+    return FD_OK;
+}
+
+// out[t] = sum_j weights[t,j] * y[slots[t,j]], terms in the order of j.  A thread owns 8 columns of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void expert_combine_kernel(const T* y, int64_t y_rows, int width, const int32_t* slots, const float* weights,
+                                                             int64_t rows, int k, T* out) {
+    const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (row >= rows) return;
+    for (int col = (blockIdx.y * blockDim.x + threadIdx.x) * 8; col < width; col += gridDim.y * blockDim.x * 8) {
+        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < k; ++j) {
+            const int32_t s = slots[row * k + j];
+            if (s < 0 || s >= y_rows) continue;
+            const float w = weights[row * k + j];
+            float v[8];
+            load8(y + (int64_t)s * width + col, width - col, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] += w * v[i];
+        }
+        store8(out + row * width + col, width - col, acc);
+    }
+}
+
+}  // namespace fd
+
+extern "C" {
+
+int fd_residual_norm(const fd_norm_args* p, void* stream) {
+    FD_REQUIRE(p, "fd_residual_norm: args is NULL");
+    FD_REQUIRE(fd::valid_dtype(p->x_dtype) && fd::valid_dtype(p->h_dtype), "fd_residual_norm: unknown element type");
+    FD_REQUIRE(p->x_dtype == p->h_dtype || p->x_dtype == FD_F32, "fd_residual_norm: x is float32 or of the block's type");
+    FD_REQUIRE(p->rows >= 0 && p->width > 0, "fd_residual_norm: bad shape [%lld, %d]", (long long)p->rows, p->width);
+    if (p->width > FD_NORM_MAX_WIDTH) {
+        fd::set_error("fd_residual_norm: rows of %d elements; at most %d are held in registers", p->width, FD_NORM_MAX_WIDTH);
+        return FD_ERR_LIMIT;
+    }
+    FD_REQUIRE(p->rows < (int64_t(1) << 31), "fd_residual_norm: too many rows");
+    if (p->rows == 0) return FD_OK;
+    FD_REQUIRE(p->x, "fd_residual_norm: x is NULL");
+    FD_REQUIRE(p->h ? p->x_out != nullptr : p->pre_weight != nullptr, "fd_residual_norm: no output asked for");
+    FD_REQUIRE(!p->pre_weight || p->u, "fd_residual_norm: u is NULL");
+    FD_REQUIRE(p->h || !(p->post_weight || p->gate || p->slots), "fd_residual_norm: post norm, gate and slots belong to h");
+    FD_REQUIRE(!p->post_bias || p->post_weight, "fd_residual_norm: post_bias without post_weight");
+    FD_REQUIRE(!p->pre_bias || p->pre_weight, "fd_residual_norm: pre_bias without pre_weight");
+    FD_REQUIRE(!p->slots || (p->weights && p->k > 0 && p->h_rows >= 0), "fd_residual_norm: slots need weights and k > 0");
+    FD_REQUIRE(!p->gate || (p->gate_rows > 0 && p->rows % p->gate_rows == 0), "fd_residual_norm: %lld gate rows do not divide %lld rows",
+               (long long)p->gate_rows, (long long)p->rows);
+    FD_REQUIRE(!p->gate || p->gate_dtype == FD_F32 || p->gate_dtype == p->h_dtype, "fd_residual_norm: gate is float32 or of the block's type");
+    FD_REQUIRE(p->gate_act >= FD_GATE_NONE && p->gate_act <= FD_GATE_TANH, "fd_residual_norm: unknown gate activation");
+    FD_REQUIRE(p->eps > 0.f, "fd_residual_norm: eps must be positive");
+    fd::NormArgs a;
+    a.x = p->x; a.h = p->h; a.gate = p->gate;
+    a.post_weight = p->post_weight; a.post_bias = p->post_bias; a.pre_weight = p->pre_weight; a.pre_bias = p->pre_bias;
+    a.weights = p->weights; a.slots = p->slots; a.x_out = p->x_out; a.u = p->u;
+    a.rows = p->rows; a.h_rows = p->slots ? p->h_rows : p->rows; a.width = p->width; a.k = p->k;
+    a.rows_per_gate = p->gate ? (int)(p->rows / p->gate_rows) : 1;
+    a.gate_f32 = p->gate_dtype == FD_F32; a.gate_act = p->gate_act; a.layer = p->layer != 0; a.scale = p->scale; a.eps = p->eps;
+    const double n = (double)p->rows * p->width;
+    const int sx = fd::dtype_bytes(p->x_dtype), sh = fd::dtype_bytes(p->h_dtype);
+    fd::ProfScope scope(fd::as_stream(stream), "residual_norm", n * 8,
+                        n * (sx + (p->h ? sx + sh * (p->slots ? p->k : 1) : 0) + (p->u ? sh : 0)));
+    return fd::with_dtype(p->h_dtype, [&](auto th) {
+        using TH = decltype(th);
+        return p->x_dtype == p->h_dtype ? fd::launch_residual_norm<TH, TH>(a, fd::as_stream(stream))
+                                        : fd::launch_residual_norm<float, TH>(a, fd::as_stream(stream));
+    });
+}
+
+int fd_expert_combine(const void* y, int dtype, int64_t y_rows, int width, const int32_t* slots, const float* weights, int64_t rows, int k,
+                      void* out, void* stream) {
+    FD_REQUIRE(fd::valid_dtype(dtype), "fd_expert_combine: unknown element type");
+    FD_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && y_rows >= 0 && width > 0 && k > 0, "fd_expert_combine: bad shape");
+    if (rows == 0) return FD_OK;
+    FD_REQUIRE(slots && weights && out && (y || y_rows == 0), "fd_expert_combine: NULL pointer");
+    const int pieces = fd::ceil_div(width, 8);
+    int bx = 1;
+    while (bx < pieces && bx < 256) bx *= 2;
+    const dim3 block(bx, 256 / bx);
+    const int gy = fd::ceil_div(pieces, bx);
+    const dim3 grid((unsigned)((rows + block.y - 1) / block.y), gy < 65535 ? gy : 65535);
+    const double n = (double)rows * width * fd::dtype_bytes(dtype);
+    fd::ProfScope scope(fd::as_stream(stream), "expert_combine", 2.0 * rows * width * k, n * (k + 1));
+    return fd::with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((fd::expert_combine_kernel<T>), grid, block, 0, fd::as_stream(stream), (const T*)y, y_rows, width, slots, weights, rows,
+                           k, (T*)out);
+        FD_LAUNCH_CHECK();
+        return FD_OK;
+    });
+}
+
+}  // extern "C"

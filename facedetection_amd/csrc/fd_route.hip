@@ -1,0 +1,241 @@
+// Route of rows to experts: the k largest logits of a row, their softmax weights, and the stable counting sort of
+// all choices by expert that lays the rows out for the grouped products (fd_expert_linear).
+//
+//   choice order: logit descending, then expert ascending; -inf, NaN and masked rows choose nothing
+//   weights[t,j] = exp(l_j - l_0) / sum, the sum over the row's choices (normalize) or over all its experts
+//   slots[t,j]   = position of the choice among all choices sorted by (expert, t);  rows[slots[t,j]] = t
+//
+// Bound by the read of the logits.  A thread owns a row: it walks the row through LDS (staged by coalesced loads, 33
+// words a row so that the walk has no bank conflicts) and keeps its k best in registers, which takes 64 rows a wave
+// where a wave-wide arg-max would take 6 cross-lane steps a choice for one row.  A row's experts are distinct, so
+// the rank of a choice among its workgroup's choices of that expert is a population count over one bit per row:
+// set with LDS atomics, whose order does not show.  Workgroups are joined by a second launch that sums their counts.
+#include "fd_elem.h"
+
+namespace fd {
+
+constexpr int ROUTE_ROWS = 512;            // rows and threads of a workgroup
+constexpr int ROUTE_COLS = 32;             // experts staged at a time
+constexpr int ROUTE_WORDS = ROUTE_ROWS / 64;
+constexpr int ROUTE_STAGE = ROUTE_ROWS * (ROUTE_COLS + 1);
+
+struct RouteArgs {
+    const void* logits;
+    const uint8_t* mask;
+    int rows, experts, k, normalize, blocks;
+    float* weights;
+    int32_t *chosen, *slots, *offsets, *source, *counts;     // counts [blocks, experts]: the workspace
+};
+
+// Exclusive scan of `v` over the workgroup's first n threads' values; every thread gets its own prefix.  Uses `words` (512 ints).
+__device__ __forceinline__ int exclusive_scan(int v, int* words) {
+    const int t = threadIdx.x;
+    words[t] = v;
+    __syncthreads();
+    for (int d = 1; d < ROUTE_ROWS; d <<= 1) {
+        const int add = t >= d ? words[t - d] : 0;
+        __syncthreads();
+        words[t] += add;
+        __syncthreads();
+    }
+    const int out = words[t] - v;
+    __syncthreads();
+    return out;
+}
+
+template <typename T, int KM>
+__global__ __launch_bounds__(ROUTE_ROWS) void expert_choose_kernel(RouteArgs a) {
+    __shared__ float stage[ROUTE_STAGE];
+    extern __shared__ unsigned long long bits[];                // [experts][ROUTE_WORDS]
+    const int t = threadIdx.x, row0 = blockIdx.x * ROUTE_ROWS, row = row0 + t;
+    const bool live = row < a.rows && (!a.mask || a.mask[row] != 0);
+    for (int i = t; i < a.experts * ROUTE_WORDS; i += ROUTE_ROWS) bits[i] = 0;
+
+    float top[KM];
+    int best[KM];
+#pragma unroll
+    for (int i = 0; i < KM; ++i) {
+        top[i] = -INFINITY;
+        best[i] = -1;
+    }
+    float sum = 0.f, sum_at = -INFINITY;           // of exp(v - sum_at) over the row so far
+    const int rows_here = min(ROUTE_ROWS, a.rows - row0);
+    for (int c0 = 0; c0 < a.experts; c0 += ROUTE_COLS) {
+        const int cols = min(ROUTE_COLS, a.experts - c0);
+        __syncthreads();
+        for (int i = t; i < rows_here * ROUTE_COLS; i += ROUTE_ROWS) {
+            const int r = i / ROUTE_COLS, c = i % ROUTE_COLS;
+            if (c < cols) stage[r * (ROUTE_COLS + 1) + c] = (float)((const T*)a.logits)[(int64_t)(row0 + r) * a.experts + c0 + c];
+        }
+        __syncthreads();
+        if (live) {
+            for (int c = 0; c < cols; ++c) {
+                const float v = stage[t * (ROUTE_COLS + 1) + c];
+                if (v > top[KM - 1]) {
+#pragma unroll
+                    for (int i = KM - 1; i >= 0; --i) {
+                        const bool here = v > top[i], above = i > 0 && v > top[i > 0 ? i - 1 : 0];
+                        top[i] = above ? top[i - 1] : (here ? v : top[i]);
+                        best[i] = above ? best[i - 1] : (here ? c0 + c : best[i]);
+                    }
+                }
+            }
+            if (!a.normalize && top[0] > -INFINITY) {
+                if (sum_at != top[0]) sum = sum_at == -INFINITY ? 0.f : sum * expf(sum_at - top[0]);
+                sum_at = top[0];
+                for (int c = 0; c < cols; ++c) {
+                    const float v = stage[t * (ROUTE_COLS + 1) + c];
+                    sum += v == sum_at ? 1.f : (v < sum_at ? expf(v - sum_at) : 0.f);
+                }
+            }
+        }
+    }
+
+    float e[KM];
+    float chosen_sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < KM; ++i) {
+        const bool is = i < a.k && best[i] >= 0;
+        e[i] = !is ? 0.f : (top[i] == top[0] ? 1.f : expf(top[i] - top[0]));
+        chosen_sum += e[i];
+        if (is) atomicOr(&bits[best[i] * ROUTE_WORDS + (t >> 6)], 1ull << (t & 63));
+    }
+    if (a.normalize) sum = chosen_sum;
+    __syncthreads();
+
+    // counts of this workgroup; with one workgroup they are the totals
+    int n = 0;
+    if (t < a.experts)
+#pragma unroll
+        for (int w = 0; w < ROUTE_WORDS; ++w) n += __popcll(bits[t * ROUTE_WORDS + w]);
+    int* base = (int*)stage;
+    if (a.blocks == 1) {
+        const int first = exclusive_scan(n, base + ROUTE_ROWS);
+        base[t] = first;
+        if (t < a.experts) a.offsets[t] = first;
+        if (t == a.experts - 1) a.offsets[a.experts] = first + n;
+        if (t == ROUTE_ROWS - 1) base[ROUTE_ROWS] = first + n;
+        __syncthreads();
+        for (int i = base[ROUTE_ROWS] + t; i < a.rows * a.k; i += ROUTE_ROWS) a.source[i] = -1;
+    } else if (t < a.experts) {
+        a.counts[(int64_t)blockIdx.x * a.experts + t] = n;
+    }
+    if (row >= a.rows) return;
+#pragma unroll
+    for (int i = 0; i < KM; ++i) {
+        if (i >= a.k) continue;
+        int at = -1;
+        if (best[i] >= 0) {
+            const unsigned long long* b = bits + best[i] * ROUTE_WORDS;
+            at = __popcll(b[t >> 6] & ((1ull << (t & 63)) - 1));
+            for (int w = 0; w < (t >> 6); ++w) at += __popcll(b[w]);
+            if (a.blocks == 1) {
+                at += base[best[i]];
+                a.source[at] = row;
+            }
+        }
+        a.weights[(int64_t)row * a.k + i] = best[i] >= 0 ? e[i] / sum : 0.f;
+        a.chosen[(int64_t)row * a.k + i] = best[i];
+        a.slots[(int64_t)row * a.k + i] = at;                  // several workgroups: the rank, placed below
+    }
+}
+
+// Adds to every choice's rank the choices of earlier experts and of earlier workgroups.
+__global__ __launch_bounds__(ROUTE_ROWS) void expert_place_kernel(RouteArgs a) {
+    __shared__ int before[ROUTE_ROWS], total[ROUTE_ROWS], words[ROUTE_ROWS];
+    const int t = threadIdx.x;
+    // 512 / lanes threads share an expert, each sums every (512 / lanes)-th workgroup
+    int lanes = 1;
+    while (lanes < a.experts) lanes *= 2;
+    const int e = t & (lanes - 1), part = t / lanes, parts = ROUTE_ROWS / lanes;
+    int b0 = 0, all = 0;
+    if (e < a.experts)
+        for (int b = part; b < a.blocks; b += parts) {
+            const int n = a.counts[(int64_t)b * a.experts + e];
+            all += n;
+            if (b < (int)blockIdx.x) b0 += n;
+        }
+    before[t] = b0;
+    total[t] = all;
+    __syncthreads();
+    b0 = all = 0;
+    if (t < a.experts)
+        for (int p = 0; p < parts; ++p) {
+            b0 += before[p * lanes + t];
+            all += total[p * lanes + t];
+        }
+    __syncthreads();
+    const int first = exclusive_scan(all, words);
+    before[t] = first + b0;
+    if (t == ROUTE_ROWS - 1) total[0] = first + all;
+    if (blockIdx.x == 0) {
+        if (t < a.experts) a.offsets[t] = first;
+        if (t == a.experts - 1) a.offsets[a.experts] = first + all;
+    }
+    __syncthreads();
+    const int row = blockIdx.x * ROUTE_ROWS + t;
+    if (row < a.rows)
+        for (int j = 0; j < a.k; ++j) {
+            const int64_t i = (int64_t)row * a.k + j;
+            const int x = a.chosen[i];
+            if (x < 0) continue;
+            const int at = before[x] + a.slots[i];
+            a.slots[i] = at;
+            a.source[at] = row;
+        }
+    const int64_t n = (int64_t)a.rows * a.k, end = (int64_t)(blockIdx.x + 1) * ROUTE_ROWS * a.k;
+    for (int64_t i = (int64_t)blockIdx.x * ROUTE_ROWS * a.k + t; i < (end < n ? end : n); i += ROUTE_ROWS)
+        if (i >= total[0]) a.source[i] = -1;
+}
+
+template <typename T>
+static void launch_choose(const RouteArgs& a, hipStream_t s) {
+    const dim3 grid(a.blocks), block(ROUTE_ROWS);
+    const size_t lds = (size_t)a.experts * ROUTE_WORDS * sizeof(unsigned long long);
+    if (a.k == 1) hipLaunchKernelGGL((expert_choose_kernel<T, 1>), grid, block, lds, s, a);
+    else if (a.k == 2) hipLaunchKernelGGL((expert_choose_kernel<T, 2>), grid, block, lds, s, a);
+    else if (a.k <= 4) hipLaunchKernelGGL((expert_choose_kernel<T, 4>), grid, block, lds, s, a);
+    else if (a.k <= 8) hipLaunchKernelGGL((expert_choose_kernel<T, 8>), grid, block, lds, s, a);
+    else hipLaunchKernelGGL((expert_choose_kernel<T, 16>), grid, block, lds, s, a);
+}
+
+}  // namespace fd
+
+extern "C" {
+
+int64_t fd_expert_route_workspace(int64_t rows, int experts) {
+    const int64_t blocks = (rows + fd::ROUTE_ROWS - 1) / fd::ROUTE_ROWS;
+    return blocks > 1 ? blocks * experts * (int64_t)sizeof(int32_t) : 0;
+}
+
+int fd_expert_route(const void* logits, int dtype, int64_t rows, int experts, int k, const uint8_t* mask, int normalize, float* weights,
+                    int32_t* chosen, int32_t* slots, int32_t* offsets, int32_t* source_rows, void* workspace, int64_t workspace_bytes,
+                    void* stream) {
+    FD_REQUIRE(fd::valid_dtype(dtype), "fd_expert_route: unknown element type");
+    FD_REQUIRE(rows >= 0 && experts > 0 && k > 0 && k <= experts, "fd_expert_route: bad shape (rows %lld, experts %d, k %d)", (long long)rows,
+               experts, k);
+    if (experts > FD_ROUTE_MAX_EXPERTS || k > FD_ROUTE_MAX_K || rows * k >= (int64_t(1) << 31) - 1024) {
+        fd::set_error("fd_expert_route: at most %d experts, %d choices a row and 2^31 - 1024 choices", FD_ROUTE_MAX_EXPERTS, FD_ROUTE_MAX_K);
+        return FD_ERR_LIMIT;
+    }
+    FD_REQUIRE(offsets && (rows == 0 || (logits && weights && chosen && slots && source_rows)), "fd_expert_route: NULL pointer");
+    FD_REQUIRE(workspace_bytes >= fd_expert_route_workspace(rows, experts) && (workspace || workspace_bytes <= 0),
+               "fd_expert_route: a workspace of %lld bytes is needed", (long long)fd_expert_route_workspace(rows, experts));
+    fd::RouteArgs a;
+    a.logits = logits; a.mask = mask; a.rows = (int)rows; a.experts = experts; a.k = k; a.normalize = normalize != 0;
+    a.blocks = rows ? fd::ceil_div(rows, fd::ROUTE_ROWS) : 1;
+    a.weights = weights; a.chosen = chosen; a.slots = slots; a.offsets = offsets; a.source = source_rows; a.counts = (int32_t*)workspace;
+    fd::ProfScope scope(fd::as_stream(stream), "expert_route", (double)rows * experts * (2 + k),
+                        (double)rows * experts * fd::dtype_bytes(dtype) + 16.0 * rows * k);
+    return fd::with_dtype(dtype, [&](auto t) {
+        fd::launch_choose<decltype(t)>(a, fd::as_stream(stream));
+        FD_LAUNCH_CHECK();
+        if (a.blocks > 1) {
+            hipLaunchKernelGGL(fd::expert_place_kernel, dim3(a.blocks), dim3(fd::ROUTE_ROWS), 0, fd::as_stream(stream), a);
+            FD_LAUNCH_CHECK();
+        }
+        return FD_OK;
+    });
+}
+
+}  // extern "C"

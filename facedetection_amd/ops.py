@@ -2,6 +2,7 @@
 reference graph calls (symbol/faster_rcnn.py:98-103) plus the detector tail
 (detection.py:47-58).  NumPy in -> NumPy out, torch in -> torch (device) out."""
 import ctypes as C
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -197,3 +198,230 @@ def crop_rects(boxes, height, width):
                                              int(b.shape[1]), n, 1, 1, None, runtime.ptr(rects),
                                              runtime.stream_ptr()))
     return None, rects.cpu().numpy()
+
+
+# ---------------------------------------------------------------------------------------------------------
+# Expert block: the operators of a residual block whose products are split over experts, on rows [T, width]
+# (rois, or positions of a channels-last map).  float32, float16 and bfloat16 rows (anything else is converted
+# to float32), float32 arithmetic.
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_ACTS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
+_GATE_ACTS = {None: 0, "sigmoid": 1, "tanh": 2}
+_NP_TYPES = {"float32": torch.float32, "float16": torch.float16}
+
+
+def _row_type(a):
+    t = a.dtype if isinstance(a, torch.Tensor) else _NP_TYPES.get(np.asarray(a).dtype.name)
+    return t if t in _DTYPES else torch.float32
+
+
+def _rows(a, index, name, dtype=None):
+    """A [rows, width] tensor on the GPU in its own type, or in ``dtype`` (another of the three types is refused)."""
+    if a.ndim != 2:
+        raise ValueError("%s must be [rows, width], not %d-dimensional" % (name, a.ndim))
+    return _typed(a, index, name, dtype)
+
+
+def _typed(a, index, name, dtype=None):
+    t = _row_type(a)
+    if dtype is not None and t != dtype:
+        if (a.dtype if isinstance(a, torch.Tensor) else _NP_TYPES.get(a.dtype.name)) in _DTYPES:
+            raise ValueError("%s is %s, %s expected" % (name, t, dtype))
+        t = dtype
+    return runtime.rows_to_device(a, t, index)
+
+
+def _ints(a, index, name):
+    """int32 indices on the GPU; a wider type is refused, since a conversion could wrap."""
+    if str(a.dtype).split(".")[-1] != "int32":
+        raise ValueError("%s must be int32, not %s" % (name, a.dtype))
+    return runtime.rows_to_device(a, torch.int32, index)
+
+
+def _params(a, index, name, width):
+    if a is None:
+        return None
+    if tuple(a.shape) != (width,):
+        raise ValueError("%s must have shape (%d,), not %s" % (name, width, tuple(a.shape)))
+    return runtime.rows_to_device(a, torch.float32, index)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class ExpertRoute(NamedTuple):
+    """What :func:`expert_route` returns (see there)."""
+    weights: object
+    experts: object
+    slots: object
+    offsets: object
+    rows: object
+
+
+def expert_route(logits, top_k, mask=None, normalize=True):
+    """Route of rows to experts.  logits [T, E] -> ExpertRoute of
+
+    * weights [T, k] float32: softmax over the row's choices, or with ``normalize=False`` over all E experts;
+    * experts [T, k] int32: the row's k largest logits, descending, equal ones by ascending expert;
+    * slots [T, k] int32: the position of each choice when all are sorted by expert, then by row;
+    * offsets [E + 1] int32: expert e has the slots offsets[e] .. offsets[e + 1] - 1;
+    * rows [T * k] int32: the row of each slot, -1 from offsets[E] on.
+
+    A logit of -inf or NaN is never chosen, and rows where ``mask`` [T] (bool or uint8) is false choose nothing; a
+    choice that is not made is -1 with weight 0.  At most 512 experts and 16 choices."""
+    as_np = not isinstance(logits, torch.Tensor)
+    index = runtime.device_index()
+    x = _rows(logits, index, "logits")
+    T, E = x.shape
+    k = int(top_k)
+    if not 0 < k <= E:
+        raise ValueError("top_k must be between 1 and the %d experts, not %d" % (E, k))
+    if mask is not None:
+        if tuple(mask.shape) != (T,) or str(mask.dtype).split(".")[-1] not in ("bool", "uint8"):
+            raise ValueError("mask must be bool or uint8 of shape (%d,)" % T)
+        mask = runtime.rows_to_device(mask, torch.bool, index)
+    L = _lib.lib()
+    empty = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=x.device)
+    weights, chosen, slots = empty((T, k), torch.float32), empty((T, k), torch.int32), empty((T, k), torch.int32)
+    offsets, source = empty((E + 1,), torch.int32), empty((T * k,), torch.int32)
+    nbytes = L.fd_expert_route_workspace(T, E)
+    work = empty((nbytes,), torch.uint8) if nbytes else None
+    _lib.check(L.fd_expert_route(x.data_ptr(), _DTYPES[x.dtype], T, E, k, _ptr(mask), 1 if normalize else 0, weights.data_ptr(),
+                                 chosen.data_ptr(), slots.data_ptr(), offsets.data_ptr(), source.data_ptr(), _ptr(work), nbytes,
+                                 runtime.stream_ptr(index)))
+    out = ExpertRoute(weights, chosen, slots, offsets, source)
+    return ExpertRoute(*(t.cpu().numpy() for t in out)) if as_np else out
+
+
+def expert_linear(x, weight, offsets, rows=None, bias=None, activation=None, gated=False):
+    """Matrix products grouped by expert: x [T, K], weight [E, N, K] -> y [S, N], S = len(rows), or T without ``rows``.
+
+    Slot s with offsets[e] <= s < offsets[e + 1] is expert e's: y[s] = act(x[rows[s]] @ weight[e].T + bias[e]), or
+    of x[s] without ``rows`` (x is in slot order then).  ``activation``: None, "relu", "silu" or "gelu" (the erf form).
+    ``gated``: weight [E, 2N, K] and bias [E, 2N] hold two halves and y[s] = act(first half) * second half.
+    ``offsets`` and ``rows`` are int32 as :func:`expert_route` gives them; slots from offsets[E] on become zeros, an
+    index of ``rows`` outside x reads as a row of zeros.  x, weight and bias are of one type, and so is y."""
+    as_np = not isinstance(x, torch.Tensor)
+    index = runtime.device_index()
+    x = _rows(x, index, "x")
+    T, K = x.shape
+    if weight.ndim != 3 or weight.shape[2] != K:
+        raise ValueError("weight must be [experts, outputs, %d], not %s" % (K, tuple(weight.shape)))
+    w = _typed(weight, index, "weight", x.dtype)
+    E, n, _ = w.shape
+    if gated and n % 2:
+        raise ValueError("a gated weight has two halves of rows, not %d rows" % n)
+    N = n // 2 if gated else n
+    if activation not in _ACTS:
+        raise ValueError("unknown activation %r" % (activation,))
+    if tuple(offsets.shape) != (E + 1,):
+        raise ValueError("offsets must have shape (%d,), not %s" % (E + 1, tuple(offsets.shape)))
+    o = _ints(offsets, index, "offsets")
+    if rows is not None:
+        if rows.ndim != 1:
+            raise ValueError("rows must be one-dimensional")
+        rows = _ints(rows, index, "rows")
+    if bias is not None:
+        if tuple(bias.shape) != (E, n):
+            raise ValueError("bias must have shape (%d, %d), not %s" % (E, n, tuple(bias.shape)))
+        bias = _typed(bias, index, "bias", x.dtype)
+    S = T if rows is None else rows.shape[0]
+    y = torch.empty((S, N), dtype=x.dtype, device=x.device)
+    _lib.check(_lib.lib().fd_expert_linear(x.data_ptr(), _DTYPES[x.dtype], T, K, w.data_ptr(), E, N, o.data_ptr(), _ptr(rows), S,
+                                           _ptr(bias), _ACTS[activation], 1 if gated else 0, y.data_ptr(), runtime.stream_ptr(index)))
+    return y.cpu().numpy() if as_np else y
+
+
+def _slots_weights(slots, weights, index, rows):
+    if slots.ndim != 2 or tuple(weights.shape) != tuple(slots.shape) or (rows is not None and slots.shape[0] != rows):
+        raise ValueError("slots and weights must both be [rows, k], not %s and %s" % (tuple(slots.shape), tuple(weights.shape)))
+    if slots.shape[1] == 0:
+        raise ValueError("slots has no columns")
+    return _ints(slots, index, "slots"), runtime.rows_to_device(weights, torch.float32, index)
+
+
+def expert_combine(y, slots, weights):
+    """Weighted sum of a row's expert outputs: y [S, N], slots / weights [T, k] -> out [T, N],
+    out[t] = sum over j of weights[t, j] * y[slots[t, j]] in the order of j.  A slot outside y (-1) adds nothing."""
+    as_np = not isinstance(y, torch.Tensor)
+    index = runtime.device_index()
+    y = _rows(y, index, "y")
+    s, w = _slots_weights(slots, weights, index, None)
+    T, k = s.shape
+    out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
+    _lib.check(_lib.lib().fd_expert_combine(y.data_ptr(), _DTYPES[y.dtype], y.shape[0], y.shape[1], s.data_ptr(), w.data_ptr(), T, k,
+                                            out.data_ptr(), runtime.stream_ptr(index)))
+    return out.cpu().numpy() if as_np else out
+
+
+def _norm_kind(kind):
+    if kind not in ("rms", "layer"):
+        raise ValueError("kind must be 'rms' or 'layer', not %r" % (kind,))
+    return 1 if kind == "layer" else 0
+
+
+def block_norm(x, weight, bias=None, kind="rms", eps=1e-6):
+    """The norm before a block: x [T, N] -> u [T, N] = x / sqrt(mean(x^2) + eps) * weight + bias, for ``kind="layer"`` of
+    x - mean(x).  weight and bias are float32 [N]."""
+    as_np = not isinstance(x, torch.Tensor)
+    index = runtime.device_index()
+    x = _rows(x, index, "x")
+    T, N = x.shape
+    weight, bias = _params(weight, index, "weight", N), _params(bias, index, "bias", N)
+    u = torch.empty_like(x)
+    t = _DTYPES[x.dtype]
+    a = _lib.NormArgs(x=x.data_ptr(), u=u.data_ptr(), pre_weight=_ptr(weight), pre_bias=_ptr(bias), rows=T, width=N, x_dtype=t, h_dtype=t,
+                      layer=_norm_kind(kind), eps=float(eps))
+    _lib.check(_lib.lib().fd_residual_norm(C.byref(a), runtime.stream_ptr(index)))
+    return u.cpu().numpy() if as_np else u
+
+
+def residual_norm(x, h, post_weight=None, post_bias=None, gate=None, gate_activation=None, scale=1.0, pre_weight=None, pre_bias=None,
+                  kind="rms", eps=1e-6, slots=None, weights=None):
+    """The end of a residual block and the start of the next: x [T, N] (the residual stream), h (the block's output) ->
+    (x', u), or x' alone without ``pre_weight``:
+
+        x' = x + scale * act(gate) * norm(h; post_weight, post_bias)        (``post_weight=None``: h as it is)
+        u  = norm(x'; pre_weight, pre_bias)
+
+    with the norms of :func:`block_norm`.  h is [T, N], or with ``slots`` and ``weights`` [T, k] an expert block's
+    [S, N], whose sum (:func:`expert_combine`) is formed on the way.  ``gate``: [N], or [G, N] with a row for each T / G
+    consecutive rows (one per frame, or with G = T one per row), float32 or of h's type; ``gate_activation``: None, "sigmoid"
+    or "tanh".  x is of h's type or float32; x' has x's type, u has h's.  Weights and biases are float32 [N]."""
+    as_np = not isinstance(x, torch.Tensor)
+    index = runtime.device_index()
+    h = _rows(h, index, "h")
+    x = _rows(x, index, "x", None if _row_type(x) == torch.float32 else h.dtype)
+    T, N = x.shape
+    if h.shape[1] != N or (slots is None and h.shape[0] != T):
+        raise ValueError("h is %s, x is %s" % (tuple(h.shape), tuple(x.shape)))
+    if (slots is None) != (weights is None):
+        raise ValueError("slots and weights come together")
+    if gate_activation not in _GATE_ACTS:
+        raise ValueError("unknown gate activation %r" % (gate_activation,))
+    if gate_activation is not None and gate is None:
+        raise ValueError("gate_activation without a gate")
+    if (post_bias is not None and post_weight is None) or (pre_bias is not None and pre_weight is None):
+        raise ValueError("a bias needs its weight")
+    a = _lib.NormArgs(x=x.data_ptr(), h=h.data_ptr(), rows=T, h_rows=h.shape[0], width=N, x_dtype=_DTYPES[x.dtype],
+                      h_dtype=_DTYPES[h.dtype], layer=_norm_kind(kind), scale=float(scale), eps=float(eps))
+    if slots is not None:
+        slots, weights = _slots_weights(slots, weights, index, T)
+        a.slots, a.weights, a.k = slots.data_ptr(), weights.data_ptr(), slots.shape[1]
+    if gate is not None:
+        if gate.ndim not in (1, 2) or gate.shape[-1] != N or (gate.ndim == 2 and (gate.shape[0] == 0 or T % gate.shape[0])):
+            raise ValueError("gate must be [%d] or [G, %d] with G a divisor of %d rows, not %s" % (N, N, T, tuple(gate.shape)))
+        gate = runtime.rows_to_device(gate, h.dtype if _row_type(gate) == h.dtype else torch.float32, index)
+        a.gate, a.gate_rows = gate.data_ptr(), gate.shape[0] if gate.ndim == 2 else 1
+        a.gate_dtype, a.gate_act = _DTYPES[gate.dtype], _GATE_ACTS[gate_activation]
+    post_weight, post_bias = _params(post_weight, index, "post_weight", N), _params(post_bias, index, "post_bias", N)
+    pre_weight, pre_bias = _params(pre_weight, index, "pre_weight", N), _params(pre_bias, index, "pre_bias", N)
+    a.post_weight, a.post_bias, a.pre_weight, a.pre_bias = _ptr(post_weight), _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias)
+    new = torch.empty_like(x)
+    u = torch.empty((T, N), dtype=h.dtype, device=x.device) if pre_weight is not None else None
+    a.x_out, a.u = new.data_ptr(), _ptr(u)
+    _lib.check(_lib.lib().fd_residual_norm(C.byref(a), runtime.stream_ptr(index)))
+    if as_np:
+        new, u = new.cpu().numpy(), None if u is None else u.cpu().numpy()
+    return new if u is None else (new, u)

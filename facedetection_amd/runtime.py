@@ -80,3 +80,12 @@ def empty(shape, dtype, device=None):
 
 def ptr(tensor):
     return C.c_void_p(tensor.data_ptr()) if tensor is not None else C.c_void_p(0)
+
+
+def rows_to_device(array, dtype, index):
+    """Contiguous tensor of ``dtype`` on GPU ``index``; one that is both already is returned as it is."""
+    if isinstance(array, torch.Tensor):
+        if array.dtype == dtype and array.is_cuda and array.get_device() == index and array.is_contiguous():
+            return array
+        return array.to(device="cuda:%d" % index, dtype=dtype).contiguous()
+    return torch.from_numpy(np.ascontiguousarray(array)).to(device="cuda:%d" % index, dtype=dtype)

@@ -338,6 +338,85 @@ int fd_detector_keep_tensors(fd_detector* det, int keep);
 int fd_detector_tensor(fd_detector* det, const char* name, float* out, int64_t capacity, int64_t* dims4,
                        void* stream);
 
+/* Expert block ------------------------------------------------------------------------------
+ * No counterpart in the reference, whose residual units (symbol/faster_rcnn.py:6-53) have one set of weights
+ * for every row: the operators of a residual block whose products are split over experts, for networks that refine the
+ * rows this path holds (rois [num_rois, 2048], positions of the feature map [H*W, 1024]).  In order of use:
+ * fd_residual_norm (norm before the block), fd_expert_route, fd_expert_linear, fd_expert_linear,
+ * fd_residual_norm (expert sum, norm after the block, gate, residual scale, norm before the next) or
+ * fd_expert_combine (the expert sum on its own).
+ * They need no context and allocate nothing (a call may be captured into a graph), operate on the CURRENT device, which
+ * the pointers and the stream belong to, and read and write rows of any length and any element alignment.  Tensors are
+ * row-major and dense.  Arithmetic is float32 with one rounding to the output's type. */
+#define FD_F32 0
+#define FD_F16 1
+#define FD_BF16 2
+
+#define FD_ROUTE_MAX_EXPERTS 512
+#define FD_ROUTE_MAX_K 16
+/* Bytes of device workspace that fd_expert_route needs (0 for up to 512 rows). */
+int64_t fd_expert_route_workspace(int64_t rows, int experts);
+/* logits [rows, experts].  Per row the k largest logits, by descending logit, equal ones by ascending expert; a logit of
+ * -inf or NaN is not chosen, a row whose mask byte (mask [rows], may be NULL) is 0 chooses nothing.
+ * weights [rows, k]: softmax over the row's choices (normalize != 0) or over all its experts; chosen [rows, k]: the experts;
+ * slots [rows, k]: the position of each choice when all choices are sorted by expert, then by row.  A choice that
+ * is not made is -1 / -1 with weight 0.  offsets [experts + 1]: expert e has the slots offsets[e] .. offsets[e+1] - 1;
+ * source_rows [rows * k]: the row of each slot, -1 from offsets[experts] on. */
+int fd_expert_route(const void* logits, int dtype, int64_t rows, int experts, int k, const uint8_t* mask, int normalize,
+                    float* weights, int32_t* chosen, int32_t* slots, int32_t* offsets, int32_t* source_rows,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+#define FD_ACT_NONE 0
+#define FD_ACT_RELU 1
+#define FD_ACT_SILU 2
+#define FD_ACT_GELU 3
+#define FD_EXPERT_MAX 1024
+/* Slot s of expert e: y[s] = act(x[r] . weight[e]^T + bias[e]), r = rows[s], or s without a row list (x_rows == slots then).
+ * x [x_rows, inner], weight [experts, outputs, inner], bias [experts, outputs] (may be NULL), y [slots, outputs], all of one
+ * type.  gated != 0: weight and bias have 2 * outputs rows, and y[s] = act(v[0 .. outputs)) * v[outputs .. 2 * outputs).
+ * offsets [experts + 1] as from fd_expert_route: offsets[0] is taken as 0, values are clamped to [the one before, slots].
+ * Slots from offsets[experts] on become zeros; an index of rows outside x reads as a row of zeros. */
+int fd_expert_linear(const void* x, int dtype, int64_t x_rows, int inner, const void* weight, int experts, int outputs,
+                     const int32_t* offsets, const int32_t* rows, int64_t slots, const void* bias, int activation, int gated,
+                     void* y, void* stream);
+
+/* out[t] = sum over j of weights[t,j] * y[slots[t,j]], in the order of j; a slot outside [0, y_rows) adds nothing.
+ * y [y_rows, width], slots / weights [rows, k], out [rows, width]. */
+int fd_expert_combine(const void* y, int dtype, int64_t y_rows, int width, const int32_t* slots, const float* weights,
+                      int64_t rows, int k, void* out, void* stream);
+
+#define FD_GATE_NONE 0
+#define FD_GATE_SIGMOID 1
+#define FD_GATE_TANH 2
+#define FD_NORM_MAX_WIDTH 16384
+/* x_out = x + scale * act(gate) * norm(h);  u = norm(x_out)   (h != NULL)
+ * u = norm(x)                                                 (h == NULL: the norm before a block)
+ * norm(v) = v / sqrt(mean(v^2) + eps) * weight + bias, or with layer != 0 of v - mean(v).  post_weight == NULL: h enters
+ * without a norm; pre_weight == NULL: u is not computed.  With slots, h is the expert sum of fd_expert_combine over
+ * h [h_rows, width].  The gate has gate_rows rows, each for rows / gate_rows consecutive rows of x (1: one for all; the number
+ * of frames: one per frame; rows: one per row).  x may be float32 beside a 16-bit h; u has h's type.  u is computed from
+ * the unrounded x_out.  x_out may be x, u may be h unless slots are given. */
+typedef struct fd_norm_args {
+    const void* x;             /* [rows, width]                                    */
+    const void* h;             /* [rows, width], with slots [h_rows, width], NULL  */
+    void* x_out;               /* [rows, width] of x's type                        */
+    void* u;                   /* [rows, width] of h's type                        */
+    const float* post_weight;  /* [width] or NULL                                  */
+    const float* post_bias;    /* [width] or NULL                                  */
+    const float* pre_weight;   /* [width] or NULL                                  */
+    const float* pre_bias;     /* [width] or NULL                                  */
+    const void* gate;          /* [gate_rows, width] or NULL                       */
+    const int32_t* slots;      /* [rows, k] or NULL                                */
+    const float* weights;      /* [rows, k], with slots                            */
+    int64_t rows, h_rows, gate_rows;
+    int width, k;
+    int x_dtype, h_dtype, gate_dtype;
+    int gate_act;              /* FD_GATE_*                                        */
+    int layer;                 /* 0: RMS norms, else layer norms                   */
+    float scale, eps;
+} fd_norm_args;
+int fd_residual_norm(const fd_norm_args* args_host, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
