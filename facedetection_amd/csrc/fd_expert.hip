@@ -3,14 +3,15 @@
 //   y[s, :] = act(x[rows[s], :] . w[e]^T + bias[e]),   offsets[e] <= s < offsets[e + 1],
 //   gated:  y[s, n] = act(v[n]) * v[N + n],  v = x . w[e]^T + bias[e] over the expert's 2N weight rows.
 //
-// The groups are ragged and known on the device only.  The grid is sized for the worst case (every group ends in a
-// partial tile); a wave finds its tile with one scan over the offsets in registers, and workgroups beyond the last tile
-// leave.  Slots behind offsets[experts] form one more group, whose tiles are zeros.
+// The groups are ragged and known on the device only.  A wave cuts them into tiles with one scan over the offsets in
+// registers; the workgroups, at most as many as the GPU holds at once, walk the tiles in that order.  Slots behind
+// offsets[experts] are zeros.
 //
 // Weights are [N, K] and rows [*, K], both with K contiguous, so both operands of a 16 x 16 matrix instruction are 16-byte
 // pieces along K: lane l holds row l & 15, piece l >> 4.  The weights are the first operand: a lane's four results are
 // then four consecutive columns of one row of y.  float32 takes four 16x16x4 instructions over the same 16 bytes (the
 // k of a lane's j-th float is the same for both operands, which is all the sum needs).  Sums are held in float32.
+#include "fd_conv_split_dev.h"
 #include "fd_elem.h"
 
 namespace fd {
@@ -33,12 +34,41 @@ template <>
 __device__ __forceinline__ f32x4_t mma<__bf16>(u32x4_t a, u32x4_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
-template <>
-__device__ __forceinline__ f32x4_t mma<float>(u32x4_t a, u32x4_t b, f32x4_t c) {
-    const f32x4_t fa = __builtin_bit_cast(f32x4_t, a), fb = __builtin_bit_cast(f32x4_t, b);
+
+// all NI x MI tiles of one 16-byte piece; in float32 the four instructions of a tile are kept apart
+template <typename T, int NI, int MI>
+__device__ __forceinline__ void mma_block(const u32x4_t (&w)[NI], const u32x4_t (&x)[MI], f32x4_t (&acc)[NI][MI]) {
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], fb[i], c, 0, 0, 0);
-    return c;
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < MI; ++j) acc[i][j] = mma<T>(w[i], x[j], acc[i][j]);
+    } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < MI; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4_t, w[i])[t], __builtin_bit_cast(f32x4_t, x[j])[t],
+                                                                     acc[i][j], 0, 0, 0);
+    }
+}
+
+// one row fragment's tiles of it
+template <typename T, int NI, int MI>
+__device__ __forceinline__ void mma_column(const u32x4_t (&w)[NI], const u32x4_t& x, f32x4_t (&acc)[NI][MI], int j) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) acc[i][j] = mma<T>(w[i], x, acc[i][j]);
+    } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4_t, w[i])[t], __builtin_bit_cast(f32x4_t, x)[t],
+                                                                 acc[i][j], 0, 0, 0);
+    }
 }
 
 // 16 bytes of a row, elements from `left` on as zeros
@@ -59,47 +89,65 @@ __device__ __forceinline__ u32x4_t load_piece(const T* p, int left) {
 
 __device__ __forceinline__ float activate(float v, int act) {
     if (act == FD_ACT_RELU) return fmaxf(v, 0.f);
-    if (act == FD_ACT_SILU) return v / (1.f + expf(-v));
+    // hardware exp2 and reciprocal, one unit each: exp(-v) is off by |v| * 2^-24 of itself, v * sigmoid(v) by less than
+    // 2^-24 * (|v| + 1) for every v, below the bound of the sum in front of it
+    if (act == FD_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * v));
     if (act == FD_ACT_GELU) return 0.5f * v * erfcf(-0.70710678118654752f * v);     // no cancellation for v << 0
     return v;
 }
 
-// The group and rows of tile `tile` when every group is cut into tiles of BM rows: expert e (experts = the unrouted rest),
-// slots [m0, m1).  Every lane of the wave takes the same number of consecutive groups; ends are clamped to [0, slots] and
-// never decrease, so any content of `offsets` stays in bounds.  False: there is no such tile.
-__device__ __forceinline__ bool find_tile(const int32_t* offsets, int experts, int slots, int bm, int tile, int& e, int& m0, int& m1) {
-    const int lane = threadIdx.x & 63, per = (experts + 64) / 64;
-    int end = 0;
-    for (int i = lane * per; i < (lane + 1) * per; ++i) end = max(end, i < experts ? min(offsets[i + 1], slots) : slots);
-    int upto = end;
+// The tiles of all groups when every group is cut into tiles of BM slots, one scan over the offsets by every wave: lane l
+// takes the same number of consecutive groups as any other, they start at slot `start` and have `tiles` tiles from
+// `first` on.  Ends are clamped to [0, slots] and never decrease, so any content of `offsets` stays in bounds.  `ends`
+// (LDS, one word a group) keeps what a lane read of its groups; all waves write the same.
+struct TileScan {
+    int start, first, tiles, total, routed;      // routed: the slots that belong to an expert
+};
+
+__device__ __forceinline__ TileScan scan_tiles(const ExpertArgs& a, int bm, int* ends) {
+    const int lane = threadIdx.x & 63, per = (a.experts + 63) / 64;
+    int upto = 0;
+    for (int i = lane * per; i < min((lane + 1) * per, a.experts); ++i) {
+        upto = max(upto, min(a.offsets[i + 1], a.slots));
+        ends[i] = upto;
+    }
+    int sum = upto;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(upto, d, 64);
-        if (lane >= d) upto = max(upto, v);
+        const int v = __shfl_up(sum, d, 64);
+        if (lane >= d) sum = max(sum, v);
     }
-    int start = __shfl_up(upto, 1, 64);
-    if (lane == 0) start = 0;
-    int tiles = 0, at = start;
-    for (int i = lane * per; i < (lane + 1) * per; ++i) {
-        const int to = max(at, i < experts ? min(offsets[i + 1], slots) : slots);
-        tiles += (to - at + bm - 1) / bm;
+    TileScan t;
+    t.routed = __builtin_amdgcn_readlane(sum, 63);
+    t.start = __shfl_up(sum, 1, 64);
+    if (lane == 0) t.start = 0;
+    t.tiles = 0;
+    int at = t.start;
+    for (int i = lane * per; i < min((lane + 1) * per, a.experts); ++i) {
+        const int to = max(at, ends[i]);
+        t.tiles += (to - at + bm - 1) / bm;
         at = to;
     }
-    int sum = tiles;
+    sum = t.tiles;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const int v = __shfl_up(sum, d, 64);
         if (lane >= d) sum += v;
     }
-    int first = sum - tiles;
-    const bool mine = tile >= first && tile < sum;
-    const unsigned long long who = __ballot(mine);
-    if (who == 0) return false;
+    t.first = sum - t.tiles;
+    t.total = __builtin_amdgcn_readlane(sum, 63);
+    return t;
+}
+
+// Tile `tile` (below the total): slots [m0, m1) of expert e.
+__device__ __forceinline__ void locate_tile(const TileScan& t, const ExpertArgs& a, const int* ends, int bm, int tile, int& e, int& m0, int& m1) {
+    const int lane = threadIdx.x & 63, per = (a.experts + 63) / 64;
+    const bool mine = tile >= t.first && tile < t.first + t.tiles;
     int fe = 0, f0 = 0, f1 = 0;
     if (mine) {
-        at = start;
-        for (int i = lane * per; i < (lane + 1) * per; ++i) {
-            const int to = max(at, i < experts ? min(offsets[i + 1], slots) : slots);
+        int at = t.start, first = t.first;
+        for (int i = lane * per; i < min((lane + 1) * per, a.experts); ++i) {
+            const int to = max(at, ends[i]);
             const int n = (to - at + bm - 1) / bm;
             if (tile >= first && tile < first + n) {
                 fe = i;
@@ -110,11 +158,36 @@ __device__ __forceinline__ bool find_tile(const int32_t* offsets, int experts, i
             at = to;
         }
     }
-    const int src = __ffsll((long long)who) - 1;
+    const int src = __ffsll((unsigned long long)__ballot(mine)) - 1;
     e = __builtin_amdgcn_readlane(fe, src);
     m0 = __builtin_amdgcn_readlane(f0, src);
     m1 = __builtin_amdgcn_readlane(f1, src);
-    return true;
+}
+
+// The tiles of this workgroup: workgroup i runs on XCD i mod 8, and each XCD walks a contiguous eighth of the tiles (columns
+// fastest), so that the tiles that share rows and weights share an L2.  The grid is a multiple of 8.
+struct TileWalk {
+    int next, end, by;
+};
+
+__device__ __forceinline__ TileWalk walk_tiles(const TileScan& t, const ExpertArgs& a) {
+    const int n = t.total * a.tiles_n, q = n >> 3, r = n & 7, xcd = blockIdx.x & 7;
+    TileWalk w;
+    const int begin = xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q;
+    w.end = begin + q + (xcd < r ? 1 : 0);
+    w.next = begin + (blockIdx.x >> 3);
+    w.by = gridDim.x >> 3;
+    return w;
+}
+
+// The slots that belong to nobody, the last ones of y, by all workgroups together.
+template <typename T>
+__device__ __forceinline__ void zero_rest(const ExpertArgs& a, int routed) {
+    const int64_t n = (int64_t)(a.slots - routed) * a.N;
+    T* p = (T*)a.y + (int64_t)routed * a.N;
+    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * blockDim.x * 8)
+        store8(p + i, (int)min<int64_t>(n - i, 8), zero);
 }
 
 // The row of x that slot s multiplies, -1 for none (a negative or too large index reads as a row of zeros).
@@ -131,35 +204,65 @@ __device__ __forceinline__ int weight_row(const ExpertArgs& a, int n0, int r) {
     return n < a.N ? ((r >> 4) & 1) * a.N + n : -1;
 }
 
-// Four results of one row and four consecutive columns, from column n on.
-template <typename T>
-__device__ __forceinline__ void store4(const ExpertArgs& a, int64_t row, int n, const float (&v)[4]) {
-    T* p = (T*)a.y + row * a.N + n;
-    if (n + 4 <= a.N) {
-        T raw[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) raw[i] = (T)v[i];
-        __builtin_memcpy(p, raw, sizeof(raw));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < a.N) p[i] = (T)v[i];
+// Results of a wave (rows from m0 on, weight rows wn .. of the tile that starts at output column n0) through `part`, the wave's
+// own piece of LDS: the float32 sums go in as they lie in registers, come back as 8 consecutive columns of a row, and
+// bias, activation, gate and the one rounding happen on the way to a full-width store.  The 16-byte piece c of row r lies
+// at c ^ (r & 15), without which the 16 rows of a write would share their banks.
+template <typename T, int NI, int MI, int BYTES>
+__device__ __forceinline__ void store_tile(const ExpertArgs& a, int e, int m0, int m1, int n0, int wn, const f32x4_t (&acc)[NI][MI], char* part) {
+    constexpr int ROW = NI * 64;                                       // bytes of a row of NI * 16 sums
+    constexpr int FIT = BYTES / (16 * ROW), JP = FIT >= MI ? MI : (FIT >= MI / 2 ? MI / 2 : MI / 4);
+    constexpr int MASK = NI * 4 - 1 < 15 ? NI * 4 - 1 : 15;
+    static_assert(JP >= 1 && JP * 16 * ROW <= BYTES && (NI & (NI - 1)) == 0, "a wave's piece of LDS holds 16 rows");
+    const int lane = threadIdx.x & 63;
+    // pieces of 8 output columns in a row; a lane stays with one of them and takes every (64 / pieces)-th row
+    const int pieces = a.gated ? NI : 2 * NI, q = lane & (pieces - 1), shift = __builtin_ctz(pieces);
+    const int n = n0 + (a.gated ? wn / 2 : wn) + q * 8, left = a.N - n;
+    const int c = a.gated ? (q >> 1) * 8 + (q & 1) * 2 : q * 2;                  // gated: 16 columns of the first half, 16 of the second
+    float b1[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, b2[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (a.bias) {
+        const T* bias = (const T*)a.bias + (int64_t)e * a.wrows + n;
+        load8(bias, left, b1);
+        if (a.gated) load8(bias + a.N, left, b2);
     }
-}
-
-// bias, activation and gate of the results of MFMA tiles (`second`: the second half's, gated only)
-template <typename T>
-__device__ __forceinline__ void finish4(const ExpertArgs& a, int e, int64_t row, int n, const f32x4_t& first, const f32x4_t& second) {
-    const T* bias = a.bias ? (const T*)a.bias + (int64_t)e * a.wrows : nullptr;
-    float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bool in = n + i < a.N;
-        float g = first[i] + (bias && in ? (float)bias[n + i] : 0.f);
-        v[i] = activate(g, a.act);
-        if (a.gated) v[i] *= second[i] + (bias && in ? (float)bias[a.N + n + i] : 0.f);
+    for (int p = 0; p < MI / JP; ++p) {
+#pragma unroll
+        for (int j = 0; j < JP; ++j)
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int r = j * 16 + (lane & 15), at = i * 4 + (lane >> 4);
+                *(f32x4_t*)(part + r * ROW + ((at ^ (r & MASK)) * 16)) = acc[i][p * JP + j];
+            }
+        for (int r = lane >> shift; r < JP * 16; r += 64 >> shift) {
+            const int m = m0 + p * JP * 16 + r;
+            if (m >= m1 || left <= 0) break;
+            auto read = [&](int at, float* to) {
+                const f32x4_t lo = *(const f32x4_t*)(part + r * ROW + ((at ^ (r & MASK)) * 16));
+                const f32x4_t hi = *(const f32x4_t*)(part + r * ROW + (((at + 1) ^ (r & MASK)) * 16));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    to[i] = lo[i];
+                    to[4 + i] = hi[i];
+                }
+            };
+            float v[8];
+            read(c, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += b1[i];
+            if (a.act) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = activate(v[i], a.act);
+            }
+            if (a.gated) {
+                float u[8];
+                read(c + 4, u);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= u[i] + b2[i];
+            }
+            store8((T*)a.y + (int64_t)m * a.N + n, left, v);
+        }
     }
-    store4<T>(a, row, n, v);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -169,18 +272,17 @@ template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256, 2) void expert_tile_kernel(ExpertArgs a) {
     constexpr int V = 16 / (int)sizeof(T), BK = 8 * V;
     constexpr int RA = BM / 32, RB = BN / 32, MI = BM / 32, NI = BN / 32;
-    __shared__ u32x4_t xs[BM * 8], ws[BN * 8];
+    __shared__ u32x4_t smem[(BM + BN) * 8];
+    u32x4_t *xs = smem, *ws = smem + BM * 8;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int tile_n = blockIdx.x % a.tiles_n;
+    __shared__ int ends[FD_EXPERT_MAX];
+    const TileScan scan = scan_tiles(a, BM, ends);
+    zero_rest<T>(a, scan.routed);
+    const TileWalk walk = walk_tiles(scan, a);
+    for (int tile = walk.next; tile < walk.end; tile += walk.by) {
     int e, m0, m1;
-    if (!find_tile(a.offsets, a.experts, a.slots, BM, blockIdx.x / a.tiles_n, e, m0, m1)) return;
-    const int n0 = tile_n * (a.gated ? BN / 2 : BN);
-    if (e == a.experts) {
-        const int n1 = min(a.N, n0 + (a.gated ? BN / 2 : BN));
-        for (int i = tid; i < (m1 - m0) * (n1 - n0); i += 256)
-            ((T*)a.y)[(int64_t)(m0 + i / (n1 - n0)) * a.N + n0 + i % (n1 - n0)] = (T)0.f;
-        return;
-    }
+    locate_tile(scan, a, ends, BM, tile / a.tiles_n, e, m0, m1);
+    const int n0 = (tile % a.tiles_n) * (a.gated ? BN / 2 : BN);
     const int c = tid & 7, r0 = tid >> 3;
     const T *xp[RA], *wp[RB];
 #pragma unroll
@@ -238,48 +340,239 @@ __global__ __launch_bounds__(256, 2) void expert_tile_kernel(ExpertArgs a) {
                 const int r = wn + i * 16 + (lane & 15);
                 wf[i] = ws[r * 8 + (piece ^ ((r >> 1) & 7))];
             }
-#pragma unroll
-            for (int i = 0; i < NI; ++i)
-#pragma unroll
-                for (int j = 0; j < MI; ++j) acc[i][j] = mma<T>(wf[i], xf[j], acc[i][j]);
+            mma_block<T>(wf, xf, acc);
         }
     }
-#pragma unroll
-    for (int j = 0; j < MI; ++j) {
-        const int s = m0 + wm + j * 16 + (lane & 15);
-        if (s >= m1) continue;
-        if (a.gated) {
-#pragma unroll
-            for (int i = 0; i < NI; i += 2) {
-                const int n = n0 + (wn + i * 16) / 2 + 4 * (lane >> 4);
-                if (n < a.N) finish4<T>(a, e, s, n, acc[i][j], acc[i + 1][j]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int n = n0 + wn + i * 16 + 4 * (lane >> 4);
-                if (n < a.N) finish4<T>(a, e, s, n, acc[i][j], acc[i][j]);
-            }
-        }
+    __syncthreads();
+    store_tile<T, NI, MI, (BM + BN) * 32>(a, e, m0 + wm, m1, n0, wn, acc, (char*)smem + wave * (BM + BN) * 32);
     }
 }
 
-// Tiles of BM slots in the worst case: every group (the unrouted rest is one more) ends in a partial tile.
-static int64_t worst_tiles(int slots, int experts, int bm) {
-    return slots / bm + (experts + 1 < slots ? experts + 1 : slots);
+// ---------------------------------------------------------------------------------------------------------------
+// The same tile with both operands loaded straight into LDS (`buffer_load_dwordx4 ... lds`): no staging registers, and
+// rows that do not exist and pieces behind K are zeros by the buffer's range check.  Needs 16-byte aligned rows and
+// 31-bit offsets, and two steps or more.  WM x WN waves, two LDS stages, one barrier a step.
+template <typename T, int BM, int BN, int WM, int WN, int OCC>
+__global__ __launch_bounds__(WM * WN * 64, OCC) void expert_dma_kernel(ExpertArgs a, unsigned x_bytes) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int WAVES = WM * WN, GA = BM / 8 / WAVES, GB = BN / 8 / WAVES, STAGE = (BM + BN) * 128;
+    constexpr int MI = BM / WM / 16, NI = BN / WN / 16, EARLY = MI >= 8 ? 1 : 0;
+    constexpr unsigned NONE = 0x80000000u;
+    static_assert(GA * WAVES * 8 == BM && GB * WAVES * 8 == BN, "whole 8-row loads a wave");
+    // one array: the compiler waits for all loads into LDS before it reads an array of its own
+    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + (FD_EXPERT_MAX + BM) * 4];
+    int *ends = (int*)(smem + 2 * STAGE), *list = ends + FD_EXPERT_MAX;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const TileScan scan = scan_tiles(a, BM, ends);
+    zero_rest<T>(a, scan.routed);
+    TileWalk walk = walk_tiles(scan, a);
+    if (walk.next >= walk.end) return;
+    const int row_bytes = a.K * (int)sizeof(T), pieces = row_bytes / 16, steps = (pieces + 7) / 8;
+    // Lane l loads 16 bytes of row l / 8 of every 8-row load, the piece that goes to position l % 8.  (r >> 1) & 7 is
+    // the same for all loads of a lane: they lie 8 * WAVES rows apart, and WAVES is even.
+    const int lrow = wave * 8 + (lane >> 3), piece = (lane & 7) ^ ((lrow >> 1) & 7);
+
+    struct Tile {
+        int e, m0, m1, n0;
+    };
+    // which tile, and a request for its part of the row list, which goes to LDS like the rows
+    auto locate = [&](int tile) {
+        Tile t;
+        locate_tile(scan, a, ends, BM, tile / a.tiles_n, t.e, t.m0, t.m1);
+        t.n0 = (tile % a.tiles_n) * (a.gated ? BN / 2 : BN);
+        if (a.rows && wave < BM / 64) {
+            const __amdgpu_buffer_rsrc_t lr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.rows + t.m0), 0, (unsigned)(t.m1 - t.m0) * 4, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(lr, (__attribute__((address_space(3))) void*)(list + wave * 64), 4, (wave * 64 + lane) * 4, 0, 0, 0);
+        }
+        return t;
+    };
+    unsigned xo[GA], wo[GB];                      // byte offset of the lane's piece of step 0, NONE for no row
+    auto address = [&](const Tile& t) {
+        const int64_t limit = a.rows ? a.x_rows : BM;
+#pragma unroll
+        for (int i = 0; i < GA; ++i) {
+            const int r = lrow + WAVES * 8 * i, src = a.rows ? list[r] : r;
+            xo[i] = src >= 0 && src < limit && t.m0 + r < t.m1 ? (unsigned)src * row_bytes + piece * 16 : NONE;
+        }
+#pragma unroll
+        for (int i = 0; i < GB; ++i) {
+            const int src = weight_row(a, t.n0, lrow + WAVES * 8 * i);
+            wo[i] = src < 0 ? NONE : (unsigned)src * row_bytes + piece * 16;
+        }
+    };
+    auto issue = [&](const Tile& t, int step, int stage) {
+        // without a row list the rows of a tile are a range of their own, so x may be of any size
+        const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.x + (a.rows ? 0 : (int64_t)t.m0 * row_bytes)), 0,
+                                                                            a.rows ? x_bytes : (unsigned)(t.m1 - t.m0) * row_bytes, 0x00020000);
+        const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.w + (int64_t)t.e * a.wrows * row_bytes), 0,
+                                                                            (unsigned)a.wrows * row_bytes, 0x00020000);
+        char* base = smem + stage * STAGE;
+        const bool none = step * 8 + piece >= pieces;
+#pragma unroll
+        for (int i = 0; i < GA; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void*)(base + (wave + WAVES * i) * 1024), 16,
+                                                     none ? NONE : xo[i], step * 128, 0, 0);
+#pragma unroll
+        for (int i = 0; i < GB; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void*)(base + BM * 128 + (wave + WAVES * i) * 1024), 16,
+                                                     none ? NONE : wo[i], step * 128, 0, 0);
+    };
+    const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+    const int frow = lane & 15, sw = (frow >> 1) & 7;
+    int xf_off[2], wf_off[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int pos = ((h * 4 + (lane >> 4)) ^ sw) * 16;
+        xf_off[h] = (wm + frow) * 128 + pos;
+        wf_off[h] = (BM + wn + frow) * 128 + pos;
+    }
+
+    // One pipeline over all steps of all tiles.  Fragments are read half a step ahead: a row fragment is replaced by that
+    // of the next half as soon as its products are issued, the weight fragments have two sets.  Early in the second
+    // half, when all of the stage has been read, the next step's data is awaited and the stage goes to the load of the step
+    // after next.  The last step of a tile leaves its stage to the results; the next tile's first step lies in the
+    // other one already.
+    u32x4_t xf[MI], wf[2][NI];
+    auto read_x = [&](int stage, int h, int j) { xf[j] = *(const u32x4_t*)(smem + stage * STAGE + xf_off[h] + j * 2048); };
+    auto read_w = [&](int stage, int h) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) wf[h][i] = *(const u32x4_t*)(smem + stage * STAGE + wf_off[h] + i * 2048);
+    };
+    Tile cur = locate(walk.next);
+    wait_vmcnt<0>();
+    pipeline_barrier();
+    address(cur);
+    issue(cur, 0, 0);
+    wait_vmcnt<0>();
+    pipeline_barrier();
+    read_w(0, 0);
+#pragma unroll
+    for (int j = 0; j < MI; ++j) read_x(0, 0, j);
+    int stage = 0;
+    for (int tile = walk.next; tile < walk.end; tile += walk.by) {
+        const bool more = tile + walk.by < walk.end;
+        Tile nxt = cur;
+        issue(cur, 1, stage ^ 1);
+        if (more) nxt = locate(tile + walk.by);
+        f32x4_t acc[NI][MI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < MI; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int step = 0; step < steps; ++step) {
+            read_w(stage, 1);
+            __builtin_amdgcn_sched_barrier(0);           // the compiler would gather the products and then wait for all reads
+#pragma unroll
+            for (int j = 0; j < MI; ++j) {
+                mma_column<T>(wf[0], xf[j], acc, j);
+                read_x(stage, 1, j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int j = 0; j < MI; ++j) {
+                mma_column<T>(wf[1], xf[j], acc, j);
+                if (j == EARLY) {
+                    wait_vmcnt<0>();
+                    pipeline_barrier();
+                    if (step + 2 < steps) {
+                        issue(cur, step + 2, stage);
+                    } else if (step + 2 == steps && more) {
+                        address(nxt);
+                        issue(nxt, 0, stage);
+                    }
+                    stage ^= 1;
+                    read_w(stage, 0);
+#pragma unroll
+                    for (int k = 0; k <= EARLY; ++k) read_x(stage, 0, k);
+                } else if (j > EARLY) {
+                    read_x(stage, 0, j);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        constexpr int PART = STAGE / WAVES;
+        store_tile<T, NI, MI, PART>(a, cur.e, cur.m0 + wm, cur.m1, cur.n0, wn, acc, smem + (stage ^ 1) * STAGE + wave * PART);
+        pipeline_barrier();
+        cur = nxt;
+    }
+#endif
+}
+
+// Tiles of BM slots in the worst case: every group ends in a partial tile.
+static int64_t worst_tiles(int slots, int experts, int bm) { return slots / bm + (experts < slots ? experts : slots); }
+
+// CUs of the current device, asked for once.
+static int compute_units() {
+    static int cus[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    if (!cus[dev] && hipDeviceGetAttribute(&cus[dev], hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 256;
+    return cus[dev];
+}
+
+// Workgroups for tiles of BM slots: as many as run at once, a multiple of the 8 XCDs; 0 with an error if the tiles cannot
+// be counted in 31 bits.
+static int tile_grid(const ExpertArgs& a, int bm, int per_cu) {
+    const int64_t most = (int64_t)compute_units() * per_cu, tiles = worst_tiles(a.slots, a.experts, bm) * a.tiles_n;
+    if (tiles >= (int64_t(1) << 31) - (1 << 20)) {
+        set_error("fd_expert_linear: more than 2^31 - 2^20 tiles");
+        return 0;
+    }
+    return (int)(((tiles < most ? tiles : most) + 7) / 8 * 8);
 }
 
 template <typename T, int BM, int BN>
 static int launch_expert_tile(ExpertArgs a, hipStream_t stream) {
     a.tiles_n = ceil_div(a.N, a.gated ? BN / 2 : BN);
-    const int64_t blocks = worst_tiles(a.slots, a.experts, BM) * a.tiles_n;
-    if (blocks >= (int64_t(1) << 31)) {
-        set_error("fd_expert_linear: too many tiles");
-        return FD_ERR_LIMIT;
-    }
-    hipLaunchKernelGGL((expert_tile_kernel<T, BM, BN>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    const int grid = tile_grid(a, BM, BM + BN > 128 ? 2 : 4);
+    if (!grid) return FD_ERR_LIMIT;
+    hipLaunchKernelGGL((expert_tile_kernel<T, BM, BN>), dim3(grid), dim3(256), 0, stream, a);
     FD_LAUNCH_CHECK();
     return FD_OK;
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int OCC>
+static int launch_expert_dma(ExpertArgs a, hipStream_t stream) {
+    a.tiles_n = ceil_div(a.N, a.gated ? BN / 2 : BN);
+    const int grid = tile_grid(a, BM, WM * WN == 8 ? 1 : OCC);
+    if (!grid) return FD_ERR_LIMIT;
+    hipLaunchKernelGGL((expert_dma_kernel<T, BM, BN, WM, WN, OCC>), dim3(grid), dim3(WM * WN * 64), 0, stream, a,
+                       (unsigned)(a.x_rows * a.K * (int64_t)sizeof(T)));
+    FD_LAUNCH_CHECK();
+    return FD_OK;
+}
+
+// rows start on 16-byte borders and their offsets have 31 bits: the operands can be loaded straight into LDS (in two steps of 128 bytes or more)
+template <typename T>
+static bool dma_rows(const ExpertArgs& a) {
+    const int64_t row = (int64_t)a.K * sizeof(T), limit = int64_t(1) << 31;
+    return row % 16 == 0 && row > 128 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0 && a.wrows * row < limit && (a.rows ? a.x_rows : 256) * row < limit;
+}
+
+// Which tile.  A CU works through ceil(tiles / CUs) of them; one step of 128 bytes of K costs a CU (measured on 32768 rows x
+// 2048 x 4096, all CUs busy) 1.8 us for 256 x 256, 0.57 us for 128 x 128, 0.37 us for 64 x 128, 0.27 us for 64 x 64
+// in bfloat16, and a 256 x 256 tile, alone on its CU, another 8 us for its ends.  Large tiles win on many rows an expert
+// (1.17 PFLOP/s against 0.94, 0.73 and 0.51), small ones when an expert has few or the last round of tiles is nearly empty
+// (600 rows to 16 experts, 1024 -> 2 x 1024: 33, 22, 20 and 20 us).  In float32 the matrix units are slow enough (1/16) that
+// every tile reaches the same rate (126 TFLOP/s) and the smallest wastes the least.
+template <typename T>
+static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
+    if (!dma_rows<T>(a)) {
+        if (a.slots < 64ll * a.experts) return launch_expert_tile<T, 64, 64>(a, stream);
+        return launch_expert_tile<T, 128, 128>(a, stream);
+    }
+    if (sizeof(T) == 4) return launch_expert_dma<T, 64, 64, 2, 2, 4>(a, stream);
+    const int steps = ceil_div((int64_t)a.K * sizeof(T), 128);
+    const double groups = a.experts < a.slots ? a.experts : a.slots;
+    auto cost = [&](int bm, int bn, double step, double ends) {
+        const double tiles = (a.slots / (double)bm + groups / 2) * ceil_div(a.wrows, bn), rounds = ceil_div((int64_t)tiles + 1, compute_units());
+        return rounds * (steps * step + ends);
+    };
+    const double c256 = cost(256, 256, 1.8, 8.0), c128 = cost(128, 128, 0.57, 1.0), c64x128 = cost(64, 128, 0.37, 0.5), c64 = cost(64, 64, 0.27, 0.3);
+    if (c256 <= c128 && c256 <= c64x128 && c256 <= c64) return launch_expert_dma<T, 256, 256, 4, 2, 2>(a, stream);
+    if (c128 <= c64x128 && c128 <= c64) return launch_expert_dma<T, 128, 128, 2, 2, 2>(a, stream);
+    if (c64x128 <= c64) return launch_expert_dma<T, 64, 128, 2, 2, 3>(a, stream);
+    return launch_expert_dma<T, 64, 64, 2, 2, 4>(a, stream);
 }
 
 }  // namespace fd
@@ -308,8 +601,7 @@ int fd_expert_linear(const void* x, int dtype, int64_t x_rows, int inner, const 
                         s * ((double)experts * a.wrows * inner + (double)x_rows * inner + (double)slots * outputs));
     return fd::with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        if (slots < 64ll * experts) return fd::launch_expert_tile<T, 64, 64>(a, fd::as_stream(stream));
-        return fd::launch_expert_tile<T, 128, 128>(a, fd::as_stream(stream));
+        return fd::launch_expert<T>(a, fd::as_stream(stream));
     });
 }
 
