@@ -35,6 +35,15 @@ __device__ __forceinline__ f32x4_t mma<__bf16>(u32x4_t a, u32x4_t b, f32x4_t c) 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
+template <typename T>
+__device__ __forceinline__ f32x4_t mma_piece(u32x4_t w, u32x4_t x, f32x4_t c) {
+    if constexpr (sizeof(T) == 2) return mma<T>(w, x, c);
+    const f32x4_t fw = __builtin_bit_cast(f32x4_t, w), fx = __builtin_bit_cast(f32x4_t, x);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[t], fx[t], c, 0, 0, 0);
+    return c;
+}
+
 // all NI x MI tiles of one 16-byte piece; in float32 the four instructions of a tile are kept apart
 template <typename T, int NI, int MI>
 __device__ __forceinline__ void mma_block(const u32x4_t (&w)[NI], const u32x4_t (&x)[MI], f32x4_t (&acc)[NI][MI]) {
@@ -266,85 +275,92 @@ __device__ __forceinline__ void store_tile(const ExpertArgs& a, int e, int m0, i
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Tile kernel: BM slots x BN weight rows, 4 waves of (BM/2) x (BN/2), 128 bytes of K a step.  A row of a step is 8
-// pieces; piece c of row r lies at c ^ ((r >> 1) & 7), which spreads the fragment reads over the LDS banks.
-template <typename T, int BM, int BN>
-__global__ __launch_bounds__(256, 2) void expert_tile_kernel(ExpertArgs a) {
-    constexpr int V = 16 / (int)sizeof(T), BK = 8 * V;
+// Tile kernel for rows of any length and alignment: BM slots x BN weight rows, 4 waves of (BM/2) x (BN/2), 128 bytes of K a
+// step, operands through registers (D steps ahead, since every load is exposed to the full latency) into two LDS stages.
+// A row of a step is 8 pieces; piece c of row r lies at c ^ ((r >> 1) & 7), which spreads the fragment reads over the banks.
+template <typename T, int BM, int BN, int D, int OCC>
+__global__ __launch_bounds__(256, OCC) void expert_tile_kernel(ExpertArgs a) {
+    constexpr int V = 16 / (int)sizeof(T), BK = 8 * V, ROWS = BM + BN;
     constexpr int RA = BM / 32, RB = BN / 32, MI = BM / 32, NI = BN / 32;
-    __shared__ u32x4_t smem[(BM + BN) * 8];
-    u32x4_t *xs = smem, *ws = smem + BM * 8;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ u32x4_t smem[2][ROWS * 8];
     __shared__ int ends[FD_EXPERT_MAX];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const TileScan scan = scan_tiles(a, BM, ends);
     zero_rest<T>(a, scan.routed);
     const TileWalk walk = walk_tiles(scan, a);
-    for (int tile = walk.next; tile < walk.end; tile += walk.by) {
-    int e, m0, m1;
-    locate_tile(scan, a, ends, BM, tile / a.tiles_n, e, m0, m1);
-    const int n0 = (tile % a.tiles_n) * (a.gated ? BN / 2 : BN);
-    const int c = tid & 7, r0 = tid >> 3;
-    const T *xp[RA], *wp[RB];
-#pragma unroll
-    for (int i = 0; i < RA; ++i) {
-        const int s = m0 + r0 + 32 * i;
-        const int64_t r = s < m1 ? source_row(a, s) : -1;
-        xp[i] = r < 0 ? nullptr : (const T*)a.x + r * a.K;
-    }
-#pragma unroll
-    for (int i = 0; i < RB; ++i) {
-        const int r = weight_row(a, n0, r0 + 32 * i);
-        wp[i] = r < 0 ? nullptr : (const T*)a.w + ((int64_t)e * a.wrows + r) * a.K;
-    }
-    f32x4_t acc[NI][MI];
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int j = 0; j < MI; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-    u32x4_t xr[RA], wr[RB];
-    auto fetch = [&](int k) {
-        const int at = k + c * V;
-#pragma unroll
-        for (int i = 0; i < RA; ++i) xr[i] = load_piece(xp[i] + at, xp[i] ? a.K - at : 0);
-#pragma unroll
-        for (int i = 0; i < RB; ++i) wr[i] = load_piece(wp[i] + at, wp[i] ? a.K - at : 0);
-    };
+    const int c = tid & 7, r0 = tid >> 3, pos = c ^ ((r0 >> 1) & 7);
     const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
-    fetch(0);
-    for (int k = 0; k < a.K; k += BK) {
-        __syncthreads();
+    const int steps = (a.K + BK - 1) / BK;
+    for (int tile = walk.next; tile < walk.end; tile += walk.by) {
+        int e, m0, m1;
+        locate_tile(scan, a, ends, BM, tile / a.tiles_n, e, m0, m1);
+        const int n0 = (tile % a.tiles_n) * (a.gated ? BN / 2 : BN);
+        // Rows that a tile does not have read as some row that exists, their results are not stored; a row that the list
+        // does not name reads as zeros.
+        const T *xp[RA], *wp[RB];
+        bool none[RA];
 #pragma unroll
         for (int i = 0; i < RA; ++i) {
-            const int r = r0 + 32 * i;
-            xs[r * 8 + (c ^ ((r >> 1) & 7))] = xr[i];
+            const int64_t r = source_row(a, min(m0 + r0 + 32 * i, m1 - 1));
+            none[i] = r < 0;
+            xp[i] = a.x_rows ? (const T*)a.x + (r < 0 ? 0 : r) * a.K : (const T*)a.w;
         }
 #pragma unroll
         for (int i = 0; i < RB; ++i) {
-            const int r = r0 + 32 * i;
-            ws[r * 8 + (c ^ ((r >> 1) & 7))] = wr[i];
+            const int r = weight_row(a, n0, r0 + 32 * i);
+            wp[i] = (const T*)a.w + ((int64_t)e * a.wrows + (r < 0 ? 0 : r)) * a.K;
+        }
+        f32x4_t acc[NI][MI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < MI; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+        u32x4_t xr[D][RA], wr[D][RB];
+        auto fetch = [&](int step, u32x4_t (&x)[RA], u32x4_t (&w)[RB]) {
+            const int at = step * BK + c * V;
+            if ((step + 1) * BK <= a.K) {
+#pragma unroll
+                for (int i = 0; i < RA; ++i) __builtin_memcpy(&x[i], xp[i] + at, 16);
+#pragma unroll
+                for (int i = 0; i < RB; ++i) __builtin_memcpy(&w[i], wp[i] + at, 16);
+            } else {
+#pragma unroll
+                for (int i = 0; i < RA; ++i) x[i] = load_piece(xp[i] + at, a.K - at);
+#pragma unroll
+                for (int i = 0; i < RB; ++i) w[i] = load_piece(wp[i] + at, a.K - at);
+            }
+        };
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (d < steps) fetch(d, xr[d], wr[d]);
+        for (int first = 0; first < steps; first += D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                const int step = first + d;
+                if (step >= steps) break;
+                u32x4_t* stage = smem[step & 1];
+#pragma unroll
+                for (int i = 0; i < RA; ++i) stage[(r0 + 32 * i) * 8 + pos] = none[i] ? u32x4_t{0, 0, 0, 0} : xr[d][i];
+#pragma unroll
+                for (int i = 0; i < RB; ++i) stage[(BM + r0 + 32 * i) * 8 + pos] = wr[d][i];
+                if (step + D < steps) fetch(step + D, xr[d], wr[d]);
+                pipeline_barrier();
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    u32x4_t xf[MI], wf[NI];
+                    const int at = (h * 4 + (lane >> 4)) ^ ((lane >> 1) & 7);
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) wf[i] = stage[(BM + wn + i * 16 + (lane & 15)) * 8 + at];
+#pragma unroll
+                    for (int j = 0; j < MI; ++j) xf[j] = stage[(wm + j * 16 + (lane & 15)) * 8 + at];
+                    mma_block<T>(wf, xf, acc);
+                }
+            }
         }
         __syncthreads();
-        if (k + BK < a.K) fetch(k + BK);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            u32x4_t xf[MI], wf[NI];
-            const int piece = h * 4 + (lane >> 4);
-#pragma unroll
-            for (int j = 0; j < MI; ++j) {
-                const int r = wm + j * 16 + (lane & 15);
-                xf[j] = xs[r * 8 + (piece ^ ((r >> 1) & 7))];
-            }
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int r = wn + i * 16 + (lane & 15);
-                wf[i] = ws[r * 8 + (piece ^ ((r >> 1) & 7))];
-            }
-            mma_block<T>(wf, xf, acc);
-        }
-    }
-    __syncthreads();
-    store_tile<T, NI, MI, (BM + BN) * 32>(a, e, m0 + wm, m1, n0, wn, acc, (char*)smem + wave * (BM + BN) * 32);
+        store_tile<T, NI, MI, ROWS * 64>(a, e, m0 + wm, m1, n0, wn, acc, (char*)smem + wave * ROWS * 64);
+        __syncthreads();
     }
 }
 
@@ -498,6 +514,94 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void expert_dma_kernel(ExpertArg
 #endif
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows an expert: the weights are the traffic and each is used once, so they go straight to registers, in any alignment.
+// A workgroup owns 16 output columns of an expert (gated: 16 of each half) for up to 16 * MT of its rows; its WAVES waves take
+// every WAVES-th 64-byte chunk of K, U chunks in flight each, and their sums meet in LDS, added in the order of the waves.
+template <typename T, int MT, int G, int WAVES, int U>
+__global__ __launch_bounds__(WAVES * 64) void expert_stream_kernel(ExpertArgs a) {
+    constexpr int V = 16 / (int)sizeof(T), CHUNK = 4 * V;
+    __shared__ f32x4_t part[WAVES][MT][G][64];
+    __shared__ int ends[FD_EXPERT_MAX];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15;
+    const TileScan scan = scan_tiles(a, 16 * MT, ends);
+    zero_rest<T>(a, scan.routed);
+    const TileWalk walk = walk_tiles(scan, a);
+    const int full = a.K / CHUNK;
+    for (int tile = walk.next; tile < walk.end; tile += walk.by) {
+        int e, m0, m1;
+        locate_tile(scan, a, ends, 16 * MT, tile / a.tiles_n, e, m0, m1);
+        const int n0 = (tile % a.tiles_n) * 16;
+        const T *wp[G], *xp[MT];
+        bool none[MT];
+#pragma unroll
+        for (int g = 0; g < G; ++g) wp[g] = (const T*)a.w + ((int64_t)e * a.wrows + g * a.N + min(n0 + r, a.N - 1)) * a.K + (lane >> 4) * V;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int64_t row = source_row(a, min(m0 + t * 16 + r, m1 - 1));
+            none[t] = row < 0;
+            xp[t] = (a.x_rows ? (const T*)a.x + (row < 0 ? 0 : row) * a.K : (const T*)a.w) + (lane >> 4) * V;
+        }
+        f32x4_t acc[MT][G];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int g = 0; g < G; ++g) acc[t][g] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        auto multiply = [&](const u32x4_t (&w)[G], u32x4_t (&x)[MT]) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                if (none[t]) x[t] = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+                for (int g = 0; g < G; ++g) acc[t][g] = mma_piece<T>(w[g], x[t], acc[t][g]);
+            }
+        };
+        int c = wave;
+        for (; c + (U - 1) * WAVES < full; c += U * WAVES) {
+            u32x4_t w[U][G], x[U][MT];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) __builtin_memcpy(&w[u][g], wp[g] + (int64_t)(c + u * WAVES) * CHUNK, 16);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) __builtin_memcpy(&x[u][t], xp[t] + (int64_t)(c + u * WAVES) * CHUNK, 16);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) multiply(w[u], x[u]);
+        }
+        for (; c * CHUNK < a.K; c += WAVES) {
+            const int left = a.K - c * CHUNK - (lane >> 4) * V;
+            u32x4_t w[G], x[MT];
+#pragma unroll
+            for (int g = 0; g < G; ++g) w[g] = load_piece(wp[g] + (int64_t)c * CHUNK, left);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) x[t] = load_piece(xp[t] + (int64_t)c * CHUNK, left);
+            multiply(w, x);
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int g = 0; g < G; ++g) part[wave][t][g][lane] = acc[t][g];
+        __syncthreads();
+        for (int i = threadIdx.x; i < MT * 256; i += WAVES * 64) {
+            const int t = i >> 8, m = m0 + t * 16 + ((i >> 4) & 15), n = n0 + (i & 15);
+            const int at = (((i >> 4) & 15) + 16 * ((i & 15) >> 2)) * 4 + (i & 3);
+            float v[G];
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                v[g] = 0.f;
+#pragma unroll
+                for (int q = 0; q < WAVES; ++q) v[g] += ((const float*)part[q][t][g])[at];
+            }
+            if (m >= m1 || n >= a.N) continue;
+            const T* bias = a.bias ? (const T*)a.bias + (int64_t)e * a.wrows + n : nullptr;
+            float out = activate(v[0] + (bias ? (float)bias[0] : 0.f), a.act);
+            if constexpr (G == 2) out *= v[1] + (bias ? (float)bias[a.N] : 0.f);
+            ((T*)a.y)[(int64_t)m * a.N + n] = (T)out;
+        }
+        __syncthreads();
+    }
+}
+
 // Tiles of BM slots in the worst case: every group ends in a partial tile.
 static int64_t worst_tiles(int slots, int experts, int bm) { return slots / bm + (experts < slots ? experts : slots); }
 
@@ -521,12 +625,12 @@ static int tile_grid(const ExpertArgs& a, int bm, int per_cu) {
     return (int)(((tiles < most ? tiles : most) + 7) / 8 * 8);
 }
 
-template <typename T, int BM, int BN>
+template <typename T, int BM, int BN, int D, int OCC>
 static int launch_expert_tile(ExpertArgs a, hipStream_t stream) {
     a.tiles_n = ceil_div(a.N, a.gated ? BN / 2 : BN);
-    const int grid = tile_grid(a, BM, BM + BN > 128 ? 2 : 4);
+    const int grid = tile_grid(a, BM, OCC);
     if (!grid) return FD_ERR_LIMIT;
-    hipLaunchKernelGGL((expert_tile_kernel<T, BM, BN>), dim3(grid), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((expert_tile_kernel<T, BM, BN, D, OCC>), dim3(grid), dim3(256), 0, stream, a);
     FD_LAUNCH_CHECK();
     return FD_OK;
 }
@@ -542,6 +646,17 @@ static int launch_expert_dma(ExpertArgs a, hipStream_t stream) {
     return FD_OK;
 }
 
+template <typename T, int MT, int WAVES, int U>
+static int launch_expert_stream(ExpertArgs a, hipStream_t stream) {
+    a.tiles_n = ceil_div(a.N, 16);
+    const int grid = tile_grid(a, 16 * MT, 32 / WAVES);
+    if (!grid) return FD_ERR_LIMIT;
+    if (a.gated) hipLaunchKernelGGL((expert_stream_kernel<T, MT, 2, WAVES, U>), dim3(grid), dim3(WAVES * 64), 0, stream, a);
+    else hipLaunchKernelGGL((expert_stream_kernel<T, MT, 1, WAVES, U>), dim3(grid), dim3(WAVES * 64), 0, stream, a);
+    FD_LAUNCH_CHECK();
+    return FD_OK;
+}
+
 // rows start on 16-byte borders and their offsets have 31 bits: the operands can be loaded straight into LDS (in two steps of 128 bytes or more)
 template <typename T>
 static bool dma_rows(const ExpertArgs& a) {
@@ -549,30 +664,45 @@ static bool dma_rows(const ExpertArgs& a) {
     return row % 16 == 0 && row > 128 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0 && a.wrows * row < limit && (a.rows ? a.x_rows : 256) * row < limit;
 }
 
-// Which tile.  A CU works through ceil(tiles / CUs) of them; one step of 128 bytes of K costs a CU (measured on 32768 rows x
-// 2048 x 4096, all CUs busy) 1.8 us for 256 x 256, 0.57 us for 128 x 128, 0.37 us for 64 x 128, 0.27 us for 64 x 64
-// in bfloat16, and a 256 x 256 tile, alone on its CU, another 8 us for its ends.  Large tiles win on many rows an expert
-// (1.17 PFLOP/s against 0.94, 0.73 and 0.51), small ones when an expert has few or the last round of tiles is nearly empty
-// (600 rows to 16 experts, 1024 -> 2 x 1024: 33, 22, 20 and 20 us).  In float32 the matrix units are slow enough (1/16) that
-// every tile reaches the same rate (126 TFLOP/s) and the smallest wastes the least.
+// Which kernel, by sizes, type and alignment (times measured in bfloat16 unless said otherwise).
+//
+// Few rows an expert: the stream kernel, for 16 rows at a time while an expert has 6 or all have 16 together (20 slots on 8
+// experts of 2 x 1024 x 2048: 14.8 us, 64 x 64 tiles 21 us; one row, 2048 x 4096: 11 against 34 us), for 32 up to 24
+// an expert (128 slots on those experts: 17.6 against 21 us; 320 slots: 31 against 24.5 us).  Long rows have eight waves a
+// workgroup (float32, the 20 slots: 31.9 us, with four 34.8 us).
+//
+// Otherwise tiles.  A CU works through ceil(tiles / CUs) of them, and one step of 128 bytes of K costs a CU (with all CUs
+// busy) 1.8 us for 256 x 256, 0.57 us for 128 x 128, 0.37 us for 64 x 128 and 0.27 us for 64 x 64; a 256 x 256 tile, alone
+// on its CU, another 8 us for its ends.  Large tiles win on many rows an expert (32768 rows, 2048 x 4096: 1.17 PFLOP/s
+// against 0.94, 0.73 and 0.51), small ones when an expert has few or the last round of tiles is nearly empty (1200 slots on
+// 16 experts of 2 x 1024 x 1024: 33, 22, 20 and 20 us).  Through registers, for rows that are not aligned, it is 1.07 us for
+// 128 x 128 and 0.41 us for 64 x 64 (62682 slots, 1448 x 1001: 394 and 583 us; 2331 slots, 333 x 1001: 34 and 17 us).
+// In float32 the matrix units are slow enough (1/16) that every tile reaches the same rate (126 TFLOP/s) and the smallest
+// wastes the least.
 template <typename T>
 static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
-    if (!dma_rows<T>(a)) {
-        if (a.slots < 64ll * a.experts) return launch_expert_tile<T, 64, 64>(a, stream);
-        return launch_expert_tile<T, 128, 128>(a, stream);
-    }
-    if (sizeof(T) == 4) return launch_expert_dma<T, 64, 64, 2, 2, 4>(a, stream);
-    const int steps = ceil_div((int64_t)a.K * sizeof(T), 128);
-    const double groups = a.experts < a.slots ? a.experts : a.slots;
+    const int64_t groups = a.experts < a.slots ? a.experts : a.slots, row_bytes = (int64_t)a.K * sizeof(T);
+    if (a.slots <= 16 || a.slots <= 6 * groups)
+        return row_bytes < 8192 ? launch_expert_stream<T, 1, 4, 4>(a, stream) : launch_expert_stream<T, 1, 8, 4>(a, stream);
+    if (a.slots <= 32 || a.slots <= 24 * groups) return launch_expert_stream<T, 2, 4, 4>(a, stream);
+    const int steps = ceil_div(row_bytes, 128);
     auto cost = [&](int bm, int bn, double step, double ends) {
-        const double tiles = (a.slots / (double)bm + groups / 2) * ceil_div(a.wrows, bn), rounds = ceil_div((int64_t)tiles + 1, compute_units());
-        return rounds * (steps * step + ends);
+        const double tiles = (a.slots / (double)bm + groups / 2.0) * ceil_div(a.wrows, bn);
+        return ceil_div((int64_t)tiles + 1, compute_units()) * (steps * step + ends);
     };
-    const double c256 = cost(256, 256, 1.8, 8.0), c128 = cost(128, 128, 0.57, 1.0), c64x128 = cost(64, 128, 0.37, 0.5), c64 = cost(64, 64, 0.27, 0.3);
-    if (c256 <= c128 && c256 <= c64x128 && c256 <= c64) return launch_expert_dma<T, 256, 256, 4, 2, 2>(a, stream);
-    if (c128 <= c64x128 && c128 <= c64) return launch_expert_dma<T, 128, 128, 2, 2, 2>(a, stream);
-    if (c64x128 <= c64) return launch_expert_dma<T, 64, 128, 2, 2, 3>(a, stream);
-    return launch_expert_dma<T, 64, 64, 2, 2, 4>(a, stream);
+    if (!dma_rows<T>(a)) {
+        if (sizeof(T) == 4 || cost(64, 64, 0.41, 0.3) <= cost(128, 128, 1.07, 1.0)) return launch_expert_tile<T, 64, 64, 2, 4>(a, stream);
+        return launch_expert_tile<T, 128, 128, 1, 2>(a, stream);
+    }
+    if constexpr (sizeof(T) == 4) {
+        return launch_expert_dma<T, 64, 64, 2, 2, 4>(a, stream);
+    } else {
+        const double c256 = cost(256, 256, 1.8, 8.0), c128 = cost(128, 128, 0.57, 1.0), c64x128 = cost(64, 128, 0.37, 0.5), c64 = cost(64, 64, 0.27, 0.3);
+        if (c256 <= c128 && c256 <= c64x128 && c256 <= c64) return launch_expert_dma<T, 256, 256, 4, 2, 2>(a, stream);
+        if (c128 <= c64x128 && c128 <= c64) return launch_expert_dma<T, 128, 128, 2, 2, 2>(a, stream);
+        if (c64x128 <= c64) return launch_expert_dma<T, 64, 128, 2, 2, 3>(a, stream);
+        return launch_expert_dma<T, 64, 64, 2, 2, 4>(a, stream);
+    }
 }
 
 }  // namespace fd

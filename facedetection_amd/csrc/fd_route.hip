@@ -27,20 +27,32 @@ struct RouteArgs {
     int32_t *chosen, *slots, *offsets, *source, *counts;     // counts [blocks, experts]: the workspace
 };
 
-// Exclusive scan of `v` over the workgroup's first n threads' values; every thread gets its own prefix.  Uses `words` (512 ints).
-__device__ __forceinline__ int exclusive_scan(int v, int* words) {
-    const int t = threadIdx.x;
-    words[t] = v;
-    __syncthreads();
-    for (int d = 1; d < ROUTE_ROWS; d <<= 1) {
-        const int add = t >= d ? words[t - d] : 0;
-        __syncthreads();
-        words[t] += add;
-        __syncthreads();
+// Exclusive scan of `v` over the workgroup's threads, in `words` (8 ints of LDS).  `all`: the sum.
+__device__ __forceinline__ int exclusive_scan(int v, int* words, int& all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int sum = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int up = __shfl_up(sum, d, 64);
+        if (lane >= d) sum += up;
     }
-    const int out = words[t] - v;
+    if (lane == 63) words[wave] = sum;
     __syncthreads();
-    return out;
+    int before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < ROUTE_WORDS; ++w) {
+        if (w < wave) before += words[w];
+        all += words[w];
+    }
+    return before + sum - v;
+}
+
+// exp(d) for d <= 0 by the hardware's exp2; what d * log2(e) lost in its rounding is put back to first order
+__device__ __forceinline__ float exp_below(float d) {
+    const float t = d * 1.44269504088896341f, lost = fmaf(d, 1.44269504088896341f, -t);
+    const float e = __builtin_amdgcn_exp2f(t);
+    return e > 0.f ? fmaf(e, lost * 0.693147180559945309f, e) : 0.f;          // d = -inf: lost is not a number
 }
 
 template <typename T, int KM>
@@ -59,33 +71,49 @@ __global__ __launch_bounds__(ROUTE_ROWS) void expert_choose_kernel(RouteArgs a) 
         best[i] = -1;
     }
     float sum = 0.f, sum_at = -INFINITY;           // of exp(v - sum_at) over the row so far
-    const int rows_here = min(ROUTE_ROWS, a.rows - row0);
+    // A thread fetches 8 experts of 4 rows, 4 threads a row; the next experts are on their way while these are walked.
+    float next[4][8];
+    auto fetch = [&](int c0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = (t >> 2) + i * (ROUTE_ROWS / 4), c = c0 + (t & 3) * 8;
+            load8((const T*)a.logits + (int64_t)(row0 + r) * a.experts + c, row0 + r < a.rows ? a.experts - c : 0, next[i]);
+        }
+    };
+    fetch(0);
     for (int c0 = 0; c0 < a.experts; c0 += ROUTE_COLS) {
         const int cols = min(ROUTE_COLS, a.experts - c0);
         __syncthreads();
-        for (int i = t; i < rows_here * ROUTE_COLS; i += ROUTE_ROWS) {
-            const int r = i / ROUTE_COLS, c = i % ROUTE_COLS;
-            if (c < cols) stage[r * (ROUTE_COLS + 1) + c] = (float)((const T*)a.logits)[(int64_t)(row0 + r) * a.experts + c0 + c];
-        }
-        __syncthreads();
-        if (live) {
-            for (int c = 0; c < cols; ++c) {
-                const float v = stage[t * (ROUTE_COLS + 1) + c];
-                if (v > top[KM - 1]) {
 #pragma unroll
-                    for (int i = KM - 1; i >= 0; --i) {
-                        const bool here = v > top[i], above = i > 0 && v > top[i > 0 ? i - 1 : 0];
-                        top[i] = above ? top[i - 1] : (here ? v : top[i]);
-                        best[i] = above ? best[i - 1] : (here ? c0 + c : best[i]);
-                    }
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) stage[((t >> 2) + i * (ROUTE_ROWS / 4)) * (ROUTE_COLS + 1) + (t & 3) * 8 + j] = next[i][j];
+        __syncthreads();
+        if (c0 + ROUTE_COLS < a.experts) fetch(c0 + ROUTE_COLS);
+        if (live) {
+            const float* mine = stage + t * (ROUTE_COLS + 1);
+#pragma unroll 4
+            for (int c = 0; c < cols; ++c) {
+                // sorted insert: an entry becomes the middle one of itself, the one above and v; equal values stay in front
+                const float raw = mine[c], v = raw > -INFINITY ? raw : -INFINITY;
+                bool here[KM];
+#pragma unroll
+                for (int i = 0; i < KM; ++i) here[i] = v > top[i];
+#pragma unroll
+                for (int i = KM - 1; i > 0; --i) {
+                    top[i] = __builtin_amdgcn_fmed3f(top[i - 1], top[i], v);
+                    best[i] = here[i - 1] ? best[i - 1] : (here[i] ? c0 + c : best[i]);
                 }
+                top[0] = fmaxf(top[0], v);
+                best[0] = here[0] ? c0 + c : best[0];
             }
             if (!a.normalize && top[0] > -INFINITY) {
                 if (sum_at != top[0]) sum = sum_at == -INFINITY ? 0.f : sum * expf(sum_at - top[0]);
                 sum_at = top[0];
+#pragma unroll 4
                 for (int c = 0; c < cols; ++c) {
-                    const float v = stage[t * (ROUTE_COLS + 1) + c];
-                    sum += v == sum_at ? 1.f : (v < sum_at ? expf(v - sum_at) : 0.f);
+                    const float v = mine[c];
+                    sum += v == sum_at ? 1.f : (v < sum_at ? exp_below(v - sum_at) : 0.f);
                 }
             }
         }
@@ -110,13 +138,13 @@ __global__ __launch_bounds__(ROUTE_ROWS) void expert_choose_kernel(RouteArgs a) 
         for (int w = 0; w < ROUTE_WORDS; ++w) n += __popcll(bits[t * ROUTE_WORDS + w]);
     int* base = (int*)stage;
     if (a.blocks == 1) {
-        const int first = exclusive_scan(n, base + ROUTE_ROWS);
+        int all;
+        const int first = exclusive_scan(n, base + ROUTE_ROWS, all);
         base[t] = first;
         if (t < a.experts) a.offsets[t] = first;
-        if (t == a.experts - 1) a.offsets[a.experts] = first + n;
-        if (t == ROUTE_ROWS - 1) base[ROUTE_ROWS] = first + n;
+        if (t == 0) a.offsets[a.experts] = all;
         __syncthreads();
-        for (int i = base[ROUTE_ROWS] + t; i < a.rows * a.k; i += ROUTE_ROWS) a.source[i] = -1;
+        for (int i = all + t; i < a.rows * a.k; i += ROUTE_ROWS) a.source[i] = -1;
     } else if (t < a.experts) {
         a.counts[(int64_t)blockIdx.x * a.experts + t] = n;
     }
@@ -142,19 +170,30 @@ __global__ __launch_bounds__(ROUTE_ROWS) void expert_choose_kernel(RouteArgs a) 
 
 // Adds to every choice's rank the choices of earlier experts and of earlier workgroups.
 __global__ __launch_bounds__(ROUTE_ROWS) void expert_place_kernel(RouteArgs a) {
-    __shared__ int before[ROUTE_ROWS], total[ROUTE_ROWS], words[ROUTE_ROWS];
+    __shared__ int before[ROUTE_ROWS], total[ROUTE_ROWS], words[ROUTE_WORDS];
     const int t = threadIdx.x;
     // 512 / lanes threads share an expert, each sums every (512 / lanes)-th workgroup
     int lanes = 1;
     while (lanes < a.experts) lanes *= 2;
     const int e = t & (lanes - 1), part = t / lanes, parts = ROUTE_ROWS / lanes;
+    // the row's first choices are asked for before the counts, whose sums they wait for
+    const int row = blockIdx.x * ROUTE_ROWS + t;
+    int c4[4], r4[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const bool is = row < a.rows && j < a.k;
+        c4[j] = is ? a.chosen[(int64_t)row * a.k + j] : -1;
+        r4[j] = is ? a.slots[(int64_t)row * a.k + j] : -1;
+    }
     int b0 = 0, all = 0;
-    if (e < a.experts)
+    if (e < a.experts) {
+#pragma unroll 16
         for (int b = part; b < a.blocks; b += parts) {
             const int n = a.counts[(int64_t)b * a.experts + e];
             all += n;
             if (b < (int)blockIdx.x) b0 += n;
         }
+    }
     before[t] = b0;
     total[t] = all;
     __syncthreads();
@@ -165,27 +204,27 @@ __global__ __launch_bounds__(ROUTE_ROWS) void expert_place_kernel(RouteArgs a) {
             all += total[p * lanes + t];
         }
     __syncthreads();
-    const int first = exclusive_scan(all, words);
+    int routed;
+    const int first = exclusive_scan(all, words, routed);
     before[t] = first + b0;
-    if (t == ROUTE_ROWS - 1) total[0] = first + all;
     if (blockIdx.x == 0) {
         if (t < a.experts) a.offsets[t] = first;
-        if (t == a.experts - 1) a.offsets[a.experts] = first + all;
+        if (t == 0) a.offsets[a.experts] = routed;
     }
     __syncthreads();
-    const int row = blockIdx.x * ROUTE_ROWS + t;
+    auto place = [&](int64_t i, int x, int rank) {
+        if (x < 0) return;
+        const int at = before[x] + rank;
+        a.slots[i] = at;
+        a.source[at] = row;
+    };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) place((int64_t)row * a.k + j, c4[j], r4[j]);
     if (row < a.rows)
-        for (int j = 0; j < a.k; ++j) {
-            const int64_t i = (int64_t)row * a.k + j;
-            const int x = a.chosen[i];
-            if (x < 0) continue;
-            const int at = before[x] + a.slots[i];
-            a.slots[i] = at;
-            a.source[at] = row;
-        }
+        for (int j = 4; j < a.k; ++j) place((int64_t)row * a.k + j, a.chosen[(int64_t)row * a.k + j], a.slots[(int64_t)row * a.k + j]);
     const int64_t n = (int64_t)a.rows * a.k, end = (int64_t)(blockIdx.x + 1) * ROUTE_ROWS * a.k;
     for (int64_t i = (int64_t)blockIdx.x * ROUTE_ROWS * a.k + t; i < (end < n ? end : n); i += ROUTE_ROWS)
-        if (i >= total[0]) a.source[i] = -1;
+        if (i >= routed) a.source[i] = -1;
 }
 
 template <typename T>

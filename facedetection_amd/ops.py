@@ -271,7 +271,7 @@ def expert_route(logits, top_k, mask=None, normalize=True):
     A logit of -inf or NaN is never chosen, and rows where ``mask`` [T] (bool or uint8) is false choose nothing; a
     choice that is not made is -1 with weight 0.  At most 512 experts and 16 choices."""
     as_np = not isinstance(logits, torch.Tensor)
-    index = runtime.device_index()
+    index, stream = runtime.current()
     x = _rows(logits, index, "logits")
     T, E = x.shape
     k = int(top_k)
@@ -282,14 +282,13 @@ def expert_route(logits, top_k, mask=None, normalize=True):
             raise ValueError("mask must be bool or uint8 of shape (%d,)" % T)
         mask = runtime.rows_to_device(mask, torch.bool, index)
     L = _lib.lib()
-    empty = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=x.device)
-    weights, chosen, slots = empty((T, k), torch.float32), empty((T, k), torch.int32), empty((T, k), torch.int32)
-    offsets, source = empty((E + 1,), torch.int32), empty((T * k,), torch.int32)
+    weights, chosen, slots = x.new_empty((T, k), dtype=torch.float32), x.new_empty((T, k), dtype=torch.int32), x.new_empty((T, k), dtype=torch.int32)
+    offsets, source = x.new_empty((E + 1,), dtype=torch.int32), x.new_empty((T * k,), dtype=torch.int32)
     nbytes = L.fd_expert_route_workspace(T, E)
-    work = empty((nbytes,), torch.uint8) if nbytes else None
+    work = x.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     _lib.check(L.fd_expert_route(x.data_ptr(), _DTYPES[x.dtype], T, E, k, _ptr(mask), 1 if normalize else 0, weights.data_ptr(),
                                  chosen.data_ptr(), slots.data_ptr(), offsets.data_ptr(), source.data_ptr(), _ptr(work), nbytes,
-                                 runtime.stream_ptr(index)))
+                                 stream))
     out = ExpertRoute(weights, chosen, slots, offsets, source)
     return ExpertRoute(*(t.cpu().numpy() for t in out)) if as_np else out
 
@@ -303,7 +302,7 @@ def expert_linear(x, weight, offsets, rows=None, bias=None, activation=None, gat
     ``offsets`` and ``rows`` are int32 as :func:`expert_route` gives them; slots from offsets[E] on become zeros, an
     index of ``rows`` outside x reads as a row of zeros.  x, weight and bias are of one type, and so is y."""
     as_np = not isinstance(x, torch.Tensor)
-    index = runtime.device_index()
+    index, stream = runtime.current()
     x = _rows(x, index, "x")
     T, K = x.shape
     if weight.ndim != 3 or weight.shape[2] != K:
@@ -327,9 +326,9 @@ def expert_linear(x, weight, offsets, rows=None, bias=None, activation=None, gat
             raise ValueError("bias must have shape (%d, %d), not %s" % (E, n, tuple(bias.shape)))
         bias = _typed(bias, index, "bias", x.dtype)
     S = T if rows is None else rows.shape[0]
-    y = torch.empty((S, N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((S, N))
     _lib.check(_lib.lib().fd_expert_linear(x.data_ptr(), _DTYPES[x.dtype], T, K, w.data_ptr(), E, N, o.data_ptr(), _ptr(rows), S,
-                                           _ptr(bias), _ACTS[activation], 1 if gated else 0, y.data_ptr(), runtime.stream_ptr(index)))
+                                           _ptr(bias), _ACTS[activation], 1 if gated else 0, y.data_ptr(), stream))
     return y.cpu().numpy() if as_np else y
 
 
@@ -345,13 +344,13 @@ def expert_combine(y, slots, weights):
     """Weighted sum of a row's expert outputs: y [S, N], slots / weights [T, k] -> out [T, N],
     out[t] = sum over j of weights[t, j] * y[slots[t, j]] in the order of j.  A slot outside y (-1) adds nothing."""
     as_np = not isinstance(y, torch.Tensor)
-    index = runtime.device_index()
+    index, stream = runtime.current()
     y = _rows(y, index, "y")
     s, w = _slots_weights(slots, weights, index, None)
     T, k = s.shape
-    out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
+    out = y.new_empty((T, y.shape[1]))
     _lib.check(_lib.lib().fd_expert_combine(y.data_ptr(), _DTYPES[y.dtype], y.shape[0], y.shape[1], s.data_ptr(), w.data_ptr(), T, k,
-                                            out.data_ptr(), runtime.stream_ptr(index)))
+                                            out.data_ptr(), stream))
     return out.cpu().numpy() if as_np else out
 
 
@@ -365,7 +364,7 @@ def block_norm(x, weight, bias=None, kind="rms", eps=1e-6):
     """The norm before a block: x [T, N] -> u [T, N] = x / sqrt(mean(x^2) + eps) * weight + bias, for ``kind="layer"`` of
     x - mean(x).  weight and bias are float32 [N]."""
     as_np = not isinstance(x, torch.Tensor)
-    index = runtime.device_index()
+    index, stream = runtime.current()
     x = _rows(x, index, "x")
     T, N = x.shape
     weight, bias = _params(weight, index, "weight", N), _params(bias, index, "bias", N)
@@ -373,7 +372,7 @@ def block_norm(x, weight, bias=None, kind="rms", eps=1e-6):
     t = _DTYPES[x.dtype]
     a = _lib.NormArgs(x=x.data_ptr(), u=u.data_ptr(), pre_weight=_ptr(weight), pre_bias=_ptr(bias), rows=T, width=N, x_dtype=t, h_dtype=t,
                       layer=_norm_kind(kind), eps=float(eps))
-    _lib.check(_lib.lib().fd_residual_norm(C.byref(a), runtime.stream_ptr(index)))
+    _lib.check(_lib.lib().fd_residual_norm(C.byref(a), stream))
     return u.cpu().numpy() if as_np else u
 
 
@@ -390,7 +389,7 @@ def residual_norm(x, h, post_weight=None, post_bias=None, gate=None, gate_activa
     consecutive rows (one per frame, or with G = T one per row), float32 or of h's type; ``gate_activation``: None, "sigmoid"
     or "tanh".  x is of h's type or float32; x' has x's type, u has h's.  Weights and biases are float32 [N]."""
     as_np = not isinstance(x, torch.Tensor)
-    index = runtime.device_index()
+    index, stream = runtime.current()
     h = _rows(h, index, "h")
     x = _rows(x, index, "x", None if _row_type(x) == torch.float32 else h.dtype)
     T, N = x.shape
@@ -419,9 +418,9 @@ def residual_norm(x, h, post_weight=None, post_bias=None, gate=None, gate_activa
     pre_weight, pre_bias = _params(pre_weight, index, "pre_weight", N), _params(pre_bias, index, "pre_bias", N)
     a.post_weight, a.post_bias, a.pre_weight, a.pre_bias = _ptr(post_weight), _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias)
     new = torch.empty_like(x)
-    u = torch.empty((T, N), dtype=h.dtype, device=x.device) if pre_weight is not None else None
+    u = h.new_empty((T, N)) if pre_weight is not None else None
     a.x_out, a.u = new.data_ptr(), _ptr(u)
-    _lib.check(_lib.lib().fd_residual_norm(C.byref(a), runtime.stream_ptr(index)))
+    _lib.check(_lib.lib().fd_residual_norm(C.byref(a), stream))
     if as_np:
         new, u = new.cpu().numpy(), None if u is None else u.cpu().numpy()
     return new if u is None else (new, u)
