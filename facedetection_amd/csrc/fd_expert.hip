@@ -14,6 +14,8 @@
 #include "fd_conv_split_dev.h"
 #include "fd_elem.h"
 
+#include <type_traits>
+
 namespace fd {
 
 struct ExpertArgs {
@@ -96,12 +98,30 @@ __device__ __forceinline__ u32x4_t load_piece(const T* p, int left) {
     return v;
 }
 
+template <typename T>
+__device__ __forceinline__ float gelu(float v) {
+    if (sizeof(T) == 4) return 0.5f * v * erfcf(-0.70710678118654752f * v);     // no cancellation for v << 0
+    // 16-bit results: Abramowitz and Stegun 7.1.26, erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), t = 1 / (1 + p z), z >= 0, to 1.5e-7
+    const float z = 0.70710678118654752f * fabsf(v), t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * z);
+    const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float half_erfc = 0.5f * poly * __builtin_amdgcn_exp2f(-1.44269504088896341f * z * z);
+    return v * (v < 0.f ? half_erfc : 1.f - half_erfc);
+}
+
+template <typename T>
 __device__ __forceinline__ float activate(float v, int act) {
     if (act == FD_ACT_RELU) return fmaxf(v, 0.f);
     // hardware exp2 and reciprocal, one unit each: exp(-v) is off by |v| * 2^-24 of itself, v * sigmoid(v) by less than
     // 2^-24 * (|v| + 1) for every v, below the bound of the sum in front of it
     if (act == FD_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * v));
-    if (act == FD_ACT_GELU) return 0.5f * v * erfcf(-0.70710678118654752f * v);     // no cancellation for v << 0
+    if (act == FD_ACT_GELU) return gelu<T>(v);
+    return v;
+}
+
+// The same value, of which the compiler knows nothing: what is computed from it stays where it stands.  Addresses that are
+// needed once a tile would otherwise be computed before the loop over tiles and held, or spilled, through all of it.
+__device__ __forceinline__ int opaque(int v) {
+    asm volatile("" : "+v"(v));
     return v;
 }
 
@@ -150,7 +170,7 @@ __device__ __forceinline__ TileScan scan_tiles(const ExpertArgs& a, int bm, int*
 
 // Tile `tile` (below the total): slots [m0, m1) of expert e.
 __device__ __forceinline__ void locate_tile(const TileScan& t, const ExpertArgs& a, const int* ends, int bm, int tile, int& e, int& m0, int& m1) {
-    const int lane = threadIdx.x & 63, per = (a.experts + 63) / 64;
+    const int lane = opaque(threadIdx.x & 63), per = (a.experts + 63) / 64;
     const bool mine = tile >= t.first && tile < t.first + t.tiles;
     int fe = 0, f0 = 0, f1 = 0;
     if (mine) {
@@ -220,10 +240,10 @@ __device__ __forceinline__ int weight_row(const ExpertArgs& a, int n0, int r) {
 template <typename T, int NI, int MI, int BYTES>
 __device__ __forceinline__ void store_tile(const ExpertArgs& a, int e, int m0, int m1, int n0, int wn, const f32x4_t (&acc)[NI][MI], char* part) {
     constexpr int ROW = NI * 64;                                       // bytes of a row of NI * 16 sums
-    constexpr int FIT = BYTES / (16 * ROW), JP = FIT >= MI ? MI : (FIT >= MI / 2 ? MI / 2 : MI / 4);
+    constexpr int FIT = BYTES / (16 * ROW), JP = FIT >= MI ? MI : (FIT >= 4 ? 4 : (FIT >= 2 ? 2 : 1));
     constexpr int MASK = NI * 4 - 1 < 15 ? NI * 4 - 1 : 15;
     static_assert(JP >= 1 && JP * 16 * ROW <= BYTES && (NI & (NI - 1)) == 0, "a wave's piece of LDS holds 16 rows");
-    const int lane = threadIdx.x & 63;
+    const int lane = opaque(threadIdx.x & 63);
     // pieces of 8 output columns in a row; a lane stays with one of them and takes every (64 / pieces)-th row
     const int pieces = a.gated ? NI : 2 * NI, q = lane & (pieces - 1), shift = __builtin_ctz(pieces);
     const int n = n0 + (a.gated ? wn / 2 : wn) + q * 8, left = a.N - n;
@@ -261,7 +281,7 @@ __device__ __forceinline__ void store_tile(const ExpertArgs& a, int e, int m0, i
             for (int i = 0; i < 8; ++i) v[i] += b1[i];
             if (a.act) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = activate(v[i], a.act);
+                for (int i = 0; i < 8; ++i) v[i] = activate<T>(v[i], a.act);
             }
             if (a.gated) {
                 float u[8];
@@ -372,7 +392,7 @@ template <typename T, int BM, int BN, int WM, int WN, int OCC>
 __global__ __launch_bounds__(WM * WN * 64, OCC) void expert_dma_kernel(ExpertArgs a, unsigned x_bytes) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int WAVES = WM * WN, GA = BM / 8 / WAVES, GB = BN / 8 / WAVES, STAGE = (BM + BN) * 128;
-    constexpr int MI = BM / WM / 16, NI = BN / WN / 16, EARLY = MI >= 8 ? 1 : 0;
+    constexpr int MI = BM / WM / 16, NI = BN / WN / 16, EARLY = 0;
     constexpr unsigned NONE = 0x80000000u;
     static_assert(GA * WAVES * 8 == BM && GB * WAVES * 8 == BN, "whole 8-row loads a wave");
     // one array: the compiler waits for all loads into LDS before it reads an array of its own
@@ -515,6 +535,242 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void expert_dma_kernel(ExpertArg
 }
 
 // ---------------------------------------------------------------------------------------------------------------
+// 256 x 256 tiles, 16-bit types, one workgroup of 2 x 4 waves a CU.  A wave's 128 x 64 sums fill 128 accumulation registers; the
+// products of a 64-byte half step of a CU are 1024 cycles of its matrix units, its fragment reads 768 and the loads into
+// LDS 256 cycles of LDS, so everything that is not a product has to run beside the products: that is what the order below
+// is for.  Measured on 32768 rows x 2048 x 4096: 1.17 PFLOP/s from memory and 1.34 when all rows lie in L2, where the large
+// library product reaches 1.33; in one burst after the barrier the loads cost a tenth of it, a burst of fragment reads
+// another.  Four stages of 64 bytes, which keep three steps on their way, measured slower (1.09): 64-byte requests to L2.
+//
+// The products of one row fragment with four weight fragments, sums in accumulation registers.  In assembly because the
+// compiler, with 128 of them and 64 registers of fragments, writes products to other registers than it adds to and spills.
+// The first instruction covers a vector write to an operand just before.
+template <typename T>
+__device__ __forceinline__ void mma_row(const u32x4_t (&w)[4], const u32x4_t& x, f32x4_t (&acc)[4]) {
+#define FD_MFMA4(OP)                                                                                                   \
+    asm volatile("s_nop 1\n" OP " %0, %4, %8, %0\n" OP " %1, %5, %8, %1\n" OP " %2, %6, %8, %2\n" OP " %3, %7, %8, %3"   \
+                 : "+a"(acc[0]), "+a"(acc[1]), "+a"(acc[2]), "+a"(acc[3])                                              \
+                 : "v"(w[0]), "v"(w[1]), "v"(w[2]), "v"(w[3]), "v"(x))
+    if constexpr (__is_same(T, __bf16)) FD_MFMA4("v_mfma_f32_16x16x32_bf16");
+    else FD_MFMA4("v_mfma_f32_16x16x32_f16");
+#undef FD_MFMA4
+}
+
+// Waits until the last of those products can be read; the compiler does not see them.
+__device__ __forceinline__ void settle(f32x4_t (&acc)[4]) {
+    asm volatile("s_nop 15\ns_nop 15" : "+a"(acc[0]), "+a"(acc[1]), "+a"(acc[2]), "+a"(acc[3])::"memory");
+}
+
+// The results of a wave of the 256 x 256 tile (128 rows from m0 on, weight rows wn .. wn + 63): bias, activation, gate and
+// rounding in registers, 16 rows at a time through the wave's 2 KB of LDS to 16-byte stores (N is a multiple of 8).
+// The loads of the next tile's first two steps are awaited before the first store, so that no later wait for loads is
+// one for stores.
+template <typename T, int ACT, bool GATED>
+__device__ __forceinline__ void store_wide(const ExpertArgs& a, int e, int m0, int m1, int n0, int wn, const f32x4_t (&acc)[8][4], char* part) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const int lane = opaque(threadIdx.x & 63), quad = lane >> 4, r = lane & 15;
+    const int first = n0 + (GATED ? wn / 2 : wn);                   // output column of the wave
+    f32x4_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // gated: tiles 0 and 2 are of the first half, 1 and 3 of the second
+        const int n = first + (GATED ? i >> 1 : i) * 16 + quad * 4;
+        b[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (a.bias && n < a.N) {
+            T raw[4];
+            __builtin_memcpy(raw, (const T*)a.bias + (int64_t)e * a.wrows + (GATED && (i & 1) ? a.N : 0) + n, sizeof(raw));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) b[i][c] = (float)raw[c];
+        }
+    }
+    wait_vmcnt<0>();
+    // a lane stores the 16-byte piece p of rows row0, row0 + ROWS, ..
+    constexpr int PIECES = GATED ? 4 : 8, ROWS = 64 / PIECES;
+    const int row0 = lane / PIECES, p = lane % PIECES, n = first + p * 8;
+    T* out = (T*)a.y + (int64_t)(m0 + row0) * a.N + n;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; i += GATED ? 2 : 1) {
+            T4 q;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float v = activate<T>(acc[j][i][c] + b[i][c], ACT);
+                if (GATED) v *= acc[j][GATED ? i + 1 : i][c] + b[GATED ? i + 1 : i][c];
+                q[c] = (T)v;
+            }
+            // 8 bytes at column i * 16 + quad * 4 (gated: i / 2 * 16): rows of PIECES pieces of 16 bytes, spread over the banks
+            const int at = (GATED ? i / 2 : i) * 2 + (quad >> 1);
+            *(T4*)(part + r * (PIECES * 16) + ((at ^ (GATED ? (r >> 2) & 3 : r & 7)) * 16) + (quad & 1) * 8) = q;
+        }
+#pragma unroll
+        for (int h = 0; h < 16 / ROWS; ++h) {
+            const int row = row0 + h * ROWS;
+            const u32x4_t q = *(const u32x4_t*)(part + row * (PIECES * 16) + ((p ^ (GATED ? (row >> 2) & 3 : row & 7)) * 16));
+            if (m0 + j * 16 + row < m1 && n < a.N) __builtin_memcpy(out + (int64_t)(j * 16 + h * ROWS) * a.N, &q, 16);
+        }
+    }
+}
+
+template <typename T, int ACT, bool GATED>
+__global__ __launch_bounds__(512, 2) void expert_wide_kernel(ExpertArgs a, unsigned x_bytes) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int BM = 256, BN = 256, WN = 4, WAVES = 8, G = BM / 8 / WAVES, STAGE = (BM + BN) * 128;
+    constexpr int MI = 8, NI = 4, EARLY = 1;
+    constexpr unsigned NONE = 0x80000000u;
+    // one array: the compiler waits for all loads into LDS before it reads an array of its own
+    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + WAVES * 2048 + (FD_EXPERT_MAX + BM) * 4];
+    int *ends = (int*)(smem + 2 * STAGE + WAVES * 2048), *list = ends + FD_EXPERT_MAX;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const TileScan scan = scan_tiles(a, BM, ends);
+    zero_rest<T>(a, scan.routed);
+    TileWalk walk = walk_tiles(scan, a);
+    if (walk.next >= walk.end) return;
+    const int row_bytes = a.K * (int)sizeof(T), pieces = row_bytes / 16, steps = (pieces + 7) / 8;
+    // Lane l loads 16 bytes of row l / 8 of every 8-row load, the piece that goes to position l % 8.  (r >> 1) & 7 is
+    // the same for all loads of a lane: they lie 8 * WAVES rows apart, and WAVES is even.
+    const int lrow = wave * 8 + (lane >> 3), piece = (lane & 7) ^ ((lrow >> 1) & 7);
+
+    struct Tile {
+        int e, m0, m1, n0;
+    };
+    // which tile, and a request for its part of the row list, which goes to LDS like the rows
+    auto locate = [&](int tile) {
+        Tile t;
+        locate_tile(scan, a, ends, BM, tile / a.tiles_n, t.e, t.m0, t.m1);
+        t.n0 = (tile % a.tiles_n) * (a.gated ? BN / 2 : BN);
+        if (a.rows && wave < BM / 64) {
+            const __amdgpu_buffer_rsrc_t lr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.rows + t.m0), 0, (unsigned)(t.m1 - t.m0) * 4, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(lr, (__attribute__((address_space(3))) void*)(list + wave * 64), 4, (wave * 64 + opaque(lane)) * 4, 0, 0, 0);
+        }
+        return t;
+    };
+    unsigned xo[G], wo[G];                      // byte offset of the lane's piece of step 0, NONE for no row
+    auto address = [&](const Tile& t) {
+        const int64_t limit = a.rows ? a.x_rows : BM;
+        const int lrow = wave * 8 + (opaque(lane) >> 3);
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            const int r = lrow + WAVES * 8 * i, src = a.rows ? list[r] : r, row = weight_row(a, t.n0, r);
+            xo[i] = src >= 0 && src < limit && t.m0 + r < t.m1 ? (unsigned)src * row_bytes + piece * 16 : NONE;
+            wo[i] = row >= 0 && t.m0 < t.m1 ? (unsigned)row * row_bytes + piece * 16 : NONE;
+        }
+    };
+    // what is loaded: a tile's rows and weights, their buffers, and whether the lane's piece of the step lies behind K
+    __amdgpu_buffer_rsrc_t xr, wr;
+    auto aim = [&](const Tile& t) {
+        // without a row list the rows of a tile are a range of their own, so x may be of any size
+        xr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.x + (a.rows ? 0 : (int64_t)t.m0 * row_bytes)), 0,
+                                               a.rows ? x_bytes : (unsigned)(t.m1 - t.m0) * row_bytes, 0x00020000);
+        wr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.w + (int64_t)t.e * a.wrows * row_bytes), 0, (unsigned)a.wrows * row_bytes,
+                                               0x00020000);
+    };
+    auto load = [&](int i, int step, int stage) {
+        char* base = smem + stage * STAGE + wave * 1024;
+        const bool none = step * 8 + piece >= pieces;
+        if (i < G)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void*)(base + WAVES * i * 1024), 16,
+                                                     none ? NONE : xo[i % G], step * 128, 0, 0);
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void*)(base + BM * 128 + WAVES * (i - G) * 1024), 16,
+                                                     none ? NONE : wo[i % G], step * 128, 0, 0);
+    };
+    auto issue = [&](int step, int stage) {
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i) load(i, step, stage);
+    };
+    const int wm = (wave / WN) * 128, wn = (wave % WN) * 64;
+    const int frow = lane & 15, sw = (frow >> 1) & 7;
+    int xf_off[2], wf_off[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int pos = ((h * 4 + (lane >> 4)) ^ sw) * 16;
+        xf_off[h] = (wm + frow) * 128 + pos;
+        wf_off[h] = (BM + wn + frow) * 128 + pos;
+    }
+
+    // One pipeline over all steps of all tiles.  Fragments are read half a step ahead: a row fragment is replaced by that
+    // of the next half as soon as its products are issued, the weight fragments have two sets.  Early in the second
+    // half, when all of the stage has been read, the next step's data is awaited and the stage goes to the load of the step
+    // after next, the next tile's at a tile's last two steps.  The results have LDS of their own.
+    u32x4_t xf[MI], wf[2][NI];
+    auto read_x = [&](int stage, int h, int j) { xf[j] = *(const u32x4_t*)(smem + stage * STAGE + xf_off[h] + j * 2048); };
+    auto read_w = [&](int stage, int h) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) wf[h][i] = *(const u32x4_t*)(smem + stage * STAGE + wf_off[h] + i * 2048);
+    };
+    Tile cur = locate(walk.next);
+    wait_vmcnt<0>();
+    pipeline_barrier();
+    address(cur);
+    aim(cur);
+    issue(0, 0);
+    issue(1, 1);
+    wait_vmcnt<0>();
+    pipeline_barrier();
+    int stage = 0;
+    // One step.  KIND 0 loads the current tile's step after next, KIND 1 (the last but one) the next tile's first, KIND 2 (the
+    // last) its second.  The loads go out between the products; one burst would hold the products up.
+    auto run = [&](auto kind, int step, const Tile& nxt, f32x4_t (&acc)[MI][NI]) {
+        constexpr int KIND = decltype(kind)::value, SLOTS = MI - 1 - EARLY, N = 2 * G;
+        read_w(stage, 1);
+        __builtin_amdgcn_sched_barrier(0);           // the compiler would gather the products and then wait for all reads
+#pragma unroll
+        for (int j = 0; j < MI; ++j) {
+            mma_row<T>(wf[0], xf[j], acc[j]);
+            read_x(stage, 1, j);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const int freed = stage;
+#pragma unroll
+        for (int j = 0; j < MI; ++j) {
+            mma_row<T>(wf[1], xf[j], acc[j]);
+            if (j == EARLY) {
+                if (step > 0) wait_vmcnt<0>();       // a tile's second step has been awaited before the stores of the tile before
+                pipeline_barrier();
+                if constexpr (KIND == 1) {
+                    address(nxt);
+                    aim(nxt);
+                }
+                stage ^= 1;
+                if constexpr (KIND < 2) {
+                    read_w(stage, 0);
+#pragma unroll
+                    for (int k = 0; k <= EARLY; ++k) read_x(stage, 0, k);
+                }
+            } else if (j > EARLY) {
+                if constexpr (KIND < 2) read_x(stage, 0, j);
+#pragma unroll
+                for (int i = (j - EARLY - 1) * N / SLOTS; i < (j - EARLY) * N / SLOTS; ++i)
+                    load(i, KIND == 0 ? step + 2 : KIND - 1, freed);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    for (int tile = walk.next; tile < walk.end; tile += walk.by) {
+        Tile nxt = {0, 0, 0, 0};                     // no tile: no rows, and loads of nothing
+        if (tile + walk.by < walk.end) nxt = locate(tile + walk.by);
+        f32x4_t acc[MI][NI];
+#pragma unroll
+        for (int j = 0; j < MI; ++j)
+#pragma unroll
+            for (int i = 0; i < NI; ++i) acc[j][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        read_w(stage, 0);
+#pragma unroll
+        for (int j = 0; j < MI; ++j) read_x(stage, 0, j);
+        for (int step = 0; step < steps - 2; ++step) run(std::integral_constant<int, 0>(), step, nxt, acc);
+        run(std::integral_constant<int, 1>(), steps - 2, nxt, acc);
+        run(std::integral_constant<int, 2>(), steps - 1, nxt, acc);
+#pragma unroll
+        for (int j = 0; j < MI; ++j) settle(acc[j]);
+        store_wide<T, ACT, GATED>(a, cur.e, cur.m0 + wm, cur.m1, cur.n0, wn, acc, smem + 2 * STAGE + wave * 2048);
+        cur = nxt;
+    }
+    wait_vmcnt<0>();
+#endif
+}
+
+// ---------------------------------------------------------------------------------------------------------------
 // Few rows an expert: the weights are the traffic and each is used once, so they go straight to registers, in any alignment.
 // A workgroup owns 16 output columns of an expert (gated: 16 of each half) for up to 16 * MT of its rows; its WAVES waves take
 // every WAVES-th 64-byte chunk of K, U chunks in flight each, and their sums meet in LDS, added in the order of the waves.
@@ -594,7 +850,7 @@ __global__ __launch_bounds__(WAVES * 64) void expert_stream_kernel(ExpertArgs a)
             }
             if (m >= m1 || n >= a.N) continue;
             const T* bias = a.bias ? (const T*)a.bias + (int64_t)e * a.wrows + n : nullptr;
-            float out = activate(v[0] + (bias ? (float)bias[0] : 0.f), a.act);
+            float out = activate<T>(v[0] + (bias ? (float)bias[0] : 0.f), a.act);
             if constexpr (G == 2) out *= v[1] + (bias ? (float)bias[a.N] : 0.f);
             ((T*)a.y)[(int64_t)m * a.N + n] = (T)out;
         }
@@ -604,6 +860,12 @@ __global__ __launch_bounds__(WAVES * 64) void expert_stream_kernel(ExpertArgs a)
 
 // Tiles of BM slots in the worst case: every group ends in a partial tile.
 static int64_t worst_tiles(int slots, int experts, int bm) { return slots / bm + (experts < slots ? experts : slots); }
+
+static double expert_flops(const ExpertArgs& a) { return 2.0 * a.slots * a.wrows * (double)a.K; }
+template <typename T>
+static double expert_bytes(const ExpertArgs& a) {
+    return (double)sizeof(T) * ((double)a.experts * a.wrows * a.K + (double)a.x_rows * a.K + (double)a.slots * a.N);
+}
 
 // CUs of the current device, asked for once.
 static int compute_units() {
@@ -630,6 +892,7 @@ static int launch_expert_tile(ExpertArgs a, hipStream_t stream) {
     a.tiles_n = ceil_div(a.N, a.gated ? BN / 2 : BN);
     const int grid = tile_grid(a, BM, OCC);
     if (!grid) return FD_ERR_LIMIT;
+    ProfScope scope(stream, "expert_tile", expert_flops(a), expert_bytes<T>(a));
     hipLaunchKernelGGL((expert_tile_kernel<T, BM, BN, D, OCC>), dim3(grid), dim3(256), 0, stream, a);
     FD_LAUNCH_CHECK();
     return FD_OK;
@@ -638,12 +901,36 @@ static int launch_expert_tile(ExpertArgs a, hipStream_t stream) {
 template <typename T, int BM, int BN, int WM, int WN, int OCC>
 static int launch_expert_dma(ExpertArgs a, hipStream_t stream) {
     a.tiles_n = ceil_div(a.N, a.gated ? BN / 2 : BN);
-    const int grid = tile_grid(a, BM, WM * WN == 8 ? 1 : OCC);
+    const int grid = tile_grid(a, BM, OCC);
     if (!grid) return FD_ERR_LIMIT;
+    ProfScope scope(stream, "expert_dma", expert_flops(a), expert_bytes<T>(a));
     hipLaunchKernelGGL((expert_dma_kernel<T, BM, BN, WM, WN, OCC>), dim3(grid), dim3(WM * WN * 64), 0, stream, a,
                        (unsigned)(a.x_rows * a.K * (int64_t)sizeof(T)));
     FD_LAUNCH_CHECK();
     return FD_OK;
+}
+
+template <typename T, int ACT>
+static int launch_expert_wide(ExpertArgs a, hipStream_t stream) {
+    a.tiles_n = ceil_div(a.N, a.gated ? 128 : 256);
+    const int grid = tile_grid(a, 256, 1);
+    if (!grid) return FD_ERR_LIMIT;
+    const unsigned x_bytes = (unsigned)(a.x_rows * a.K * (int64_t)sizeof(T));
+    ProfScope scope(stream, "expert_wide", expert_flops(a), expert_bytes<T>(a));
+    if (a.gated) hipLaunchKernelGGL((expert_wide_kernel<T, ACT, true>), dim3(grid), dim3(512), 0, stream, a, x_bytes);
+    else hipLaunchKernelGGL((expert_wide_kernel<T, ACT, false>), dim3(grid), dim3(512), 0, stream, a, x_bytes);
+    FD_LAUNCH_CHECK();
+    return FD_OK;
+}
+
+template <typename T>
+static int launch_expert_wide(const ExpertArgs& a, hipStream_t stream) {
+    switch (a.act) {
+        case FD_ACT_RELU: return launch_expert_wide<T, FD_ACT_RELU>(a, stream);
+        case FD_ACT_SILU: return launch_expert_wide<T, FD_ACT_SILU>(a, stream);
+        case FD_ACT_GELU: return launch_expert_wide<T, FD_ACT_GELU>(a, stream);
+        default: return launch_expert_wide<T, FD_ACT_NONE>(a, stream);
+    }
 }
 
 template <typename T, int MT, int WAVES, int U>
@@ -651,6 +938,7 @@ static int launch_expert_stream(ExpertArgs a, hipStream_t stream) {
     a.tiles_n = ceil_div(a.N, 16);
     const int grid = tile_grid(a, 16 * MT, 32 / WAVES);
     if (!grid) return FD_ERR_LIMIT;
+    ProfScope scope(stream, "expert_stream", expert_flops(a), expert_bytes<T>(a));
     if (a.gated) hipLaunchKernelGGL((expert_stream_kernel<T, MT, 2, WAVES, U>), dim3(grid), dim3(WAVES * 64), 0, stream, a);
     else hipLaunchKernelGGL((expert_stream_kernel<T, MT, 1, WAVES, U>), dim3(grid), dim3(WAVES * 64), 0, stream, a);
     FD_LAUNCH_CHECK();
@@ -672,13 +960,13 @@ static bool dma_rows(const ExpertArgs& a) {
 // workgroup (float32, the 20 slots: 31.9 us, with four 34.8 us).
 //
 // Otherwise tiles.  A CU works through ceil(tiles / CUs) of them, and one step of 128 bytes of K costs a CU (with all CUs
-// busy) 1.8 us for 256 x 256, 0.57 us for 128 x 128, 0.37 us for 64 x 128 and 0.27 us for 64 x 64; a 256 x 256 tile, alone
-// on its CU, another 8 us for its ends.  Large tiles win on many rows an expert (32768 rows, 2048 x 4096: 1.17 PFLOP/s
+// busy) 1.75 us for 256 x 256, 0.57 us for 128 x 128, 0.37 us for 64 x 128 and 0.27 us for 64 x 64; a 256 x 256 tile, alone
+// on its CU, another 4.5 us for its ends.  Large tiles win on many rows an expert (32768 rows, 2048 x 4096: 1.17 PFLOP/s
 // against 0.94, 0.73 and 0.51), small ones when an expert has few or the last round of tiles is nearly empty (1200 slots on
-// 16 experts of 2 x 1024 x 1024: 33, 22, 20 and 20 us).  Through registers, for rows that are not aligned, it is 1.07 us for
-// 128 x 128 and 0.41 us for 64 x 64 (62682 slots, 1448 x 1001: 394 and 583 us; 2331 slots, 333 x 1001: 34 and 17 us).
-// In float32 the matrix units are slow enough (1/16) that every tile reaches the same rate (126 TFLOP/s) and the smallest
-// wastes the least.
+// 16 experts of 2 x 1024 x 1024: 33, 22, 20 and 20 us).  The largest takes outputs in eights and three steps or more.
+// Through registers, for rows that are not aligned, it is 1.07 us for 128 x 128 and 0.41 us for 64 x 64 (62682 slots,
+// 1448 x 1001: 394 and 583 us; 2331 slots, 333 x 1001: 34 and 17 us).  In float32 the matrix units are slow enough (1/16)
+// that every tile reaches the same rate (126 TFLOP/s) and the smallest wastes the least.
 template <typename T>
 static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
     const int64_t groups = a.experts < a.slots ? a.experts : a.slots, row_bytes = (int64_t)a.K * sizeof(T);
@@ -697,8 +985,8 @@ static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
     if constexpr (sizeof(T) == 4) {
         return launch_expert_dma<T, 64, 64, 2, 2, 4>(a, stream);
     } else {
-        const double c256 = cost(256, 256, 1.8, 8.0), c128 = cost(128, 128, 0.57, 1.0), c64x128 = cost(64, 128, 0.37, 0.5), c64 = cost(64, 64, 0.27, 0.3);
-        if (c256 <= c128 && c256 <= c64x128 && c256 <= c64) return launch_expert_dma<T, 256, 256, 4, 2, 2>(a, stream);
+        const double c256 = cost(256, 256, 1.75, 4.5), c128 = cost(128, 128, 0.57, 1.0), c64x128 = cost(64, 128, 0.37, 0.5), c64 = cost(64, 64, 0.27, 0.3);
+        if (a.N % 8 == 0 && row_bytes > 256 && c256 <= c128 && c256 <= c64x128 && c256 <= c64) return launch_expert_wide<T>(a, stream);
         if (c128 <= c64x128 && c128 <= c64) return launch_expert_dma<T, 128, 128, 2, 2, 2>(a, stream);
         if (c64x128 <= c64) return launch_expert_dma<T, 64, 128, 2, 2, 3>(a, stream);
         return launch_expert_dma<T, 64, 64, 2, 2, 4>(a, stream);
@@ -726,9 +1014,6 @@ int fd_expert_linear(const void* x, int dtype, int64_t x_rows, int inner, const 
     a.x = x; a.w = weight; a.bias = bias; a.y = y; a.offsets = offsets; a.rows = rows; a.x_rows = x_rows;
     a.K = inner; a.N = outputs; a.wrows = outputs * (gated ? 2 : 1); a.experts = experts; a.slots = (int)slots; a.act = activation;
     a.gated = gated != 0; a.tiles_n = 0;
-    const double s = fd::dtype_bytes(dtype);
-    fd::ProfScope scope(fd::as_stream(stream), "expert_linear", 2.0 * slots * a.wrows * (double)inner,
-                        s * ((double)experts * a.wrows * inner + (double)x_rows * inner + (double)slots * outputs));
     return fd::with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         return fd::launch_expert<T>(a, fd::as_stream(stream));

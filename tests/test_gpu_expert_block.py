@@ -225,6 +225,49 @@ def test_expert_linear(dtype, case):
     assert bool((y[int(offsets[-1]):] == 0).all())
 
 
+def _kernels(call):
+    """(result, names of the kernels a call ran)"""
+    from facedetection_amd import profiling
+    profiling.begin()
+    try:
+        out = call()
+        torch.cuda.synchronize()
+    finally:
+        rows = profiling.end()
+    return out, {r["kernel"] for r in rows}
+
+
+# large enough for the 256 x 256 tiles: ragged groups, partial tiles in both directions, a partial last step of K, several
+# tiles a workgroup, an empty expert; every activation with and without a gate
+WIDE = [
+    (50000, 2, 3, 200, 1032, "silu", True, True, True, 0.7, 0.1),
+    (100000, 1, 3, 264, 2056, None, False, False, True, 0.7, 0.0),
+    (100000, 1, 5, 328, 1040, "gelu", False, True, False, 1.0, 0.05),
+    (60000, 1, 2, 1000, 1040, "relu", True, False, False, 0.3, 0.0),
+    (30000, 4, 10, 512, 768, None, True, True, True, 0.0, 0.02),
+    (130560, 1, 1, 264, 2048, "relu", False, True, True, 0.0, 0.01),
+    (32000, 2, 4, 320, 1024, "gelu", True, False, True, 2.0, 0.0),
+    (65536, 1, 1, 512, 2056, "silu", False, False, False, 0.0, 0.0),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("case", WIDE, ids=lambda c: "x".join(str(v) for v in c[:5]))
+def test_expert_linear_largest_tiles(dtype, case):
+    from facedetection_amd import ops
+    T, k, E, K, N, act, gated, has_bias, gather, skew, drop = case
+    g = _gen(T + 7 * E + K)
+    rows, offsets, _, _ = _routing(g, T, E, k, skew, drop)
+    n = 2 * N if gated else N
+    x = torch.randn((T if gather else T * k, K), generator=g, device="cuda").to(dtype)
+    w = (torch.randn((E, n, K), generator=g, device="cuda") / math.sqrt(K)).to(dtype)
+    bias = torch.randn((E, n), generator=g, device="cuda").to(dtype) if has_bias else None
+    y, kernels = _kernels(lambda: ops.expert_linear(x, w, offsets, rows=rows if gather else None, bias=bias, activation=act, gated=gated))
+    assert kernels == {"expert_wide"}
+    _close(y, *_linear64(x, w, offsets, rows if gather else None, bias, act, gated))
+    assert bool((y[int(offsets[-1]):] == 0).all())
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_expert_linear_unaligned_views(dtype):
     """x, weight and bias that start one element past a 16-byte border, and x as a slice of wider rows."""
