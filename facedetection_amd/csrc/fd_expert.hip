@@ -433,25 +433,31 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void expert_dma_kernel(ExpertArg
 #pragma unroll
         for (int i = 0; i < GB; ++i) {
             const int src = weight_row(a, t.n0, lrow + WAVES * 8 * i);
-            wo[i] = src < 0 ? NONE : (unsigned)src * row_bytes + piece * 16;
+            wo[i] = src < 0 || t.m0 >= t.m1 ? NONE : (unsigned)src * row_bytes + piece * 16;
         }
     };
-    auto issue = [&](const Tile& t, int step, int stage) {
+    // what is loaded: a tile's rows and weights, their buffers, and whether the lane's piece of the step lies behind K
+    __amdgpu_buffer_rsrc_t xr, wr;
+    auto aim = [&](const Tile& t) {
         // without a row list the rows of a tile are a range of their own, so x may be of any size
-        const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.x + (a.rows ? 0 : (int64_t)t.m0 * row_bytes)), 0,
-                                                                            a.rows ? x_bytes : (unsigned)(t.m1 - t.m0) * row_bytes, 0x00020000);
-        const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.w + (int64_t)t.e * a.wrows * row_bytes), 0,
-                                                                            (unsigned)a.wrows * row_bytes, 0x00020000);
-        char* base = smem + stage * STAGE;
+        xr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.x + (a.rows ? 0 : (int64_t)t.m0 * row_bytes)), 0,
+                                               a.rows ? x_bytes : (unsigned)(t.m1 - t.m0) * row_bytes, 0x00020000);
+        wr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.w + (int64_t)t.e * a.wrows * row_bytes), 0, (unsigned)a.wrows * row_bytes,
+                                               0x00020000);
+    };
+    auto load = [&](int i, int step, int stage) {
+        char* base = smem + stage * STAGE + wave * 1024;
         const bool none = step * 8 + piece >= pieces;
+        if (i < GA)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void*)(base + WAVES * i * 1024), 16,
+                                                     none ? NONE : xo[i < GA ? i : 0], step * 128, 0, 0);
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void*)(base + BM * 128 + WAVES * (i - GA) * 1024), 16,
+                                                     none ? NONE : wo[i >= GA ? i - GA : 0], step * 128, 0, 0);
+    };
+    auto issue = [&](int step, int stage) {
 #pragma unroll
-        for (int i = 0; i < GA; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void*)(base + (wave + WAVES * i) * 1024), 16,
-                                                     none ? NONE : xo[i], step * 128, 0, 0);
-#pragma unroll
-        for (int i = 0; i < GB; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void*)(base + BM * 128 + (wave + WAVES * i) * 1024), 16,
-                                                     none ? NONE : wo[i], step * 128, 0, 0);
+        for (int i = 0; i < GA + GB; ++i) load(i, step, stage);
     };
     const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
     const int frow = lane & 15, sw = (frow >> 1) & 7;
@@ -478,59 +484,68 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void expert_dma_kernel(ExpertArg
     wait_vmcnt<0>();
     pipeline_barrier();
     address(cur);
-    issue(cur, 0, 0);
+    aim(cur);
+    issue(0, 0);
     wait_vmcnt<0>();
     pipeline_barrier();
     read_w(0, 0);
 #pragma unroll
     for (int j = 0; j < MI; ++j) read_x(0, 0, j);
     int stage = 0;
+    // One step.  KIND 0 loads the current tile's step after next, KIND 1 (the last but one) the next tile's first, KIND 2 (the
+    // last) nothing: its stage is left to the results.  The loads go out between the products.
+    auto run = [&](auto kind, int step, const Tile& nxt, f32x4_t (&acc)[NI][MI]) {
+        constexpr int KIND = decltype(kind)::value, SLOTS = MI - 1 - EARLY, N = GA + GB;
+        read_w(stage, 1);
+        __builtin_amdgcn_sched_barrier(0);           // the compiler would gather the products and then wait for all reads
+#pragma unroll
+        for (int j = 0; j < MI; ++j) {
+            mma_column<T>(wf[0], xf[j], acc, j);
+            read_x(stage, 1, j);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const int freed = stage;
+#pragma unroll
+        for (int j = 0; j < MI; ++j) {
+            mma_column<T>(wf[1], xf[j], acc, j);
+            if (j == EARLY) {
+                wait_vmcnt<0>();
+                pipeline_barrier();
+                if constexpr (KIND == 1) {
+                    address(nxt);
+                    aim(nxt);
+                }
+                stage ^= 1;
+                read_w(stage, 0);
+#pragma unroll
+                for (int k = 0; k <= EARLY; ++k) read_x(stage, 0, k);
+            } else if (j > EARLY) {
+                read_x(stage, 0, j);
+                if constexpr (KIND < 2)
+#pragma unroll
+                    for (int i = (j - EARLY - 1) * N / SLOTS; i < (j - EARLY) * N / SLOTS; ++i) load(i, KIND == 0 ? step + 2 : 0, freed);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
     for (int tile = walk.next; tile < walk.end; tile += walk.by) {
-        const bool more = tile + walk.by < walk.end;
-        Tile nxt = cur;
-        issue(cur, 1, stage ^ 1);
-        if (more) nxt = locate(tile + walk.by);
+        issue(1, stage ^ 1);
+        Tile nxt = {0, 0, 0, 0};                     // no tile: no rows, and loads of nothing
+        if (tile + walk.by < walk.end) nxt = locate(tile + walk.by);
         f32x4_t acc[NI][MI];
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int j = 0; j < MI; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        for (int step = 0; step < steps; ++step) {
-            read_w(stage, 1);
-            __builtin_amdgcn_sched_barrier(0);           // the compiler would gather the products and then wait for all reads
-#pragma unroll
-            for (int j = 0; j < MI; ++j) {
-                mma_column<T>(wf[0], xf[j], acc, j);
-                read_x(stage, 1, j);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int j = 0; j < MI; ++j) {
-                mma_column<T>(wf[1], xf[j], acc, j);
-                if (j == EARLY) {
-                    wait_vmcnt<0>();
-                    pipeline_barrier();
-                    if (step + 2 < steps) {
-                        issue(cur, step + 2, stage);
-                    } else if (step + 2 == steps && more) {
-                        address(nxt);
-                        issue(nxt, 0, stage);
-                    }
-                    stage ^= 1;
-                    read_w(stage, 0);
-#pragma unroll
-                    for (int k = 0; k <= EARLY; ++k) read_x(stage, 0, k);
-                } else if (j > EARLY) {
-                    read_x(stage, 0, j);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
+        for (int step = 0; step < steps - 2; ++step) run(std::integral_constant<int, 0>(), step, nxt, acc);
+        run(std::integral_constant<int, 1>(), steps - 2, nxt, acc);
+        run(std::integral_constant<int, 2>(), steps - 1, nxt, acc);
         constexpr int PART = STAGE / WAVES;
         store_tile<T, NI, MI, PART>(a, cur.e, cur.m0 + wm, cur.m1, cur.n0, wn, acc, smem + (stage ^ 1) * STAGE + wave * PART);
         pipeline_barrier();
         cur = nxt;
     }
+    wait_vmcnt<0>();
 #endif
 }
 
