@@ -24,33 +24,49 @@ inline int with_dtype(int t, F&& f) {
     }
 }
 
-// 8 elements from p as float32; elements from `n` on are zero and not read
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
-    if (n >= 8) {
-        T raw[8];
+// P elements from p as float32; elements from `n` on are zero and not read
+template <int P, typename T>
+__device__ __forceinline__ void load_elems(const T* p, int n, float (&v)[P]) {
+    if (n >= P) {
+        T raw[P];
         __builtin_memcpy(raw, p, sizeof(raw));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)raw[i];
+        for (int i = 0; i < P; ++i) v[i] = (float)raw[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+        for (int i = 0; i < P; ++i) v[i] = i < n ? (float)p[i] : 0.f;
     }
 }
 
 // the one rounding to fewer bits: to nearest even, at the end of the operator
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
-    if (n >= 8) {
-        T raw[8];
+template <int P, typename T>
+__device__ __forceinline__ void store_elems(T* p, int n, const float (&v)[P]) {
+    if (n >= P) {
+        T raw[P];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) raw[i] = (T)v[i];
+        for (int i = 0; i < P; ++i) raw[i] = (T)v[i];
         __builtin_memcpy(p, raw, sizeof(raw));
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < P; ++i)
             if (i < n) p[i] = (T)v[i];
     }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+    load_elems<8>(p, n, v);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
+    store_elems<8>(p, n, v);
+}
+
+// exp(d) by the hardware's exp2; what d * log2(e) lost in its rounding is put back to first order
+__device__ __forceinline__ float exp_fast(float d) {
+    const float t = d * 1.44269504088896341f, lost = fmaf(d, 1.44269504088896341f, -t);
+    const float e = __builtin_amdgcn_exp2f(t);
+    return e > 0.f && e < INFINITY ? fmaf(e, lost * 0.693147180559945309f, e) : e;      // at the ends `lost` is no number
 }
 
 }  // namespace fd

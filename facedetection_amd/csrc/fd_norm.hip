@@ -24,7 +24,7 @@ struct NormArgs {
 };
 
 __device__ __forceinline__ float gate_value(float g, int act) {
-    if (act == FD_GATE_SIGMOID) return 1.f / (1.f + expf(-g));
+    if (act == FD_GATE_SIGMOID) return __builtin_amdgcn_rcpf(1.f + exp_fast(-g));
     if (act == FD_GATE_TANH) return tanhf(g);
     return g;
 }
@@ -44,126 +44,189 @@ __device__ __forceinline__ float row_sum(float v, float (*part)[4], int& turn) {
     return v;
 }
 
-template <int G, int NC>
-__device__ __forceinline__ void normalise(float (&v)[NC][8], const float* weight, const float* bias, const NormArgs& a, int lane,
-                                          float (*part)[4], int& turn) {
+// weight and bias of a lane's pieces
+template <int NC, int P>
+struct NormParams {
+    float weight[NC][P], bias[NC][P];
+};
+
+template <int G, int NC, int P>
+__device__ __forceinline__ void load_params(NormParams<NC, P>& p, const float* weight, const float* bias, const NormArgs& a, int lane) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int col = (c * G + lane) * P;
+        load_elems<P>(weight + col, a.width - col, p.weight[c]);
+        if (bias) load_elems<P>(bias + col, a.width - col, p.bias[c]);
+        else
+#pragma unroll
+            for (int i = 0; i < P; ++i) p.bias[c][i] = 0.f;
+    }
+}
+
+template <int G, int NC, int P>
+__device__ __forceinline__ void normalise(float (&v)[NC][P], const NormParams<NC, P>& p, const NormArgs& a, int lane, float (*part)[4], int& turn) {
     if (a.layer) {
         float s = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[c][i];
+            for (int i = 0; i < P; ++i) s += v[c][i];
         const float mean = row_sum<G>(s, part, turn) / (float)a.width;
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c) {
+            const int left = a.width - (c * G + lane) * P;         // elements behind the row stay zero
+            if (left >= P) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if ((c * G + lane) * 8 + i < a.width) v[c][i] -= mean;
+                for (int i = 0; i < P; ++i) v[c][i] -= mean;
+            } else {
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+                    if (i < left) v[c][i] -= mean;
+            }
+        }
     }
     float s = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += v[c][i] * v[c][i];
+        for (int i = 0; i < P; ++i) s += v[c][i] * v[c][i];
     const float r = rsqrtf(row_sum<G>(s, part, turn) / (float)a.width + a.eps);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int col = (c * G + lane) * 8;
-        float w[8], b[8];
-        load8(weight + col, a.width - col, w);
-        if (bias) load8(bias + col, a.width - col, b);
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[c][i] = v[c][i] * r * w[i] + (bias ? b[i] : 0.f);
-    }
+        for (int i = 0; i < P; ++i) v[c][i] = v[c][i] * r * p.weight[c][i] + p.bias[c][i];
 }
 
-// G lanes hold a row, NC pieces of 8 elements each: element (c * G + lane) * 8 + i.
-template <typename TX, typename TH, int G, int NC>
+// Two of a row's choices, so that both rows are on their way before either is added; -1 for a choice that is not made.
+struct ChoicePair {
+    int32_t slot[2];
+    float weight[2];
+};
+
+__device__ __forceinline__ ChoicePair choice_pair(const int32_t* slots, const float* weights, int k, int j, int64_t rows) {
+    ChoicePair p;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int at = j + q < k ? j + q : j;
+        p.slot[q] = slots[at];
+        p.weight[q] = weights[at];
+        if (j + q >= k || p.slot[q] < 0 || p.slot[q] >= rows) p.slot[q] = -1;
+    }
+    return p;
+}
+
+// G lanes hold a row, NE elements each, in pieces of P: element (c * G + lane) * P + i.  A piece is 16 bytes of x, 4 elements
+// of a float32 x and 8 otherwise, so that neighbouring lanes read neighbouring pieces.  With 8 elements a lane there are
+// registers to ask for everything that the row needs before the first sum is waited for.
+template <typename TX>
+__host__ __device__ constexpr int piece_elems() {
+    return 16 / (int)sizeof(TX);
+}
+
+template <typename TX, typename TH, int G, int NE>
 __global__ __launch_bounds__(256) void residual_norm_kernel(NormArgs a) {
+    constexpr int P = piece_elems<TX>(), NC = NE / P;
     __shared__ float part[2][4];
     int turn = 0;
     const int lane = threadIdx.x % G;
     const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
     if (row >= a.rows) return;                       // a whole group of G lanes: G = 256 never leaves early
-    float x[NC][8];
+    float x[NC][P];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int col = (c * G + lane) * 8;
-        load8((const TX*)a.x + row * a.width + col, a.width - col, x[c]);
+        const int col = (c * G + lane) * P;
+        load_elems<P>((const TX*)a.x + row * a.width + col, a.width - col, x[c]);
+    }
+    const int64_t gate_row = a.gate ? (row / a.rows_per_gate) * a.width : 0;
+    NormParams<NC, P> post, pre;
+    float gate[NC][P];
+    auto load_gate = [&](int c) {
+        const int col = (c * G + lane) * P;
+        if (a.gate_f32) load_elems<P>((const float*)a.gate + gate_row + col, a.width - col, gate[c]);
+        else load_elems<P>((const TH*)a.gate + gate_row + col, a.width - col, gate[c]);
+    };
+    constexpr bool AHEAD = NE == 8;
+    if (AHEAD) {
+        if (a.post_weight) load_params<G, NC, P>(post, a.post_weight, a.post_bias, a, lane);
+        if (a.pre_weight) load_params<G, NC, P>(pre, a.pre_weight, a.pre_bias, a, lane);
+        if (a.gate)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) load_gate(c);
     }
     if (a.h) {
-        float h[NC][8];
+        float h[NC][P];
         if (a.slots) {
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) h[c][i] = 0.f;
-            for (int j = 0; j < a.k; ++j) {
-                const int32_t s = a.slots[row * a.k + j];
-                if (s < 0 || s >= a.h_rows) continue;
-                const float w = a.weights[row * a.k + j];
+                for (int i = 0; i < P; ++i) h[c][i] = 0.f;
+            for (int j = 0; j < a.k; j += 2) {
+                const ChoicePair p = choice_pair(a.slots + row * a.k, a.weights + row * a.k, a.k, j, a.h_rows);
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const int col = (c * G + lane) * 8;
-                    float y[8];
-                    load8((const TH*)a.h + (int64_t)s * a.width + col, a.width - col, y);
+                for (int q = 0; q < 2; ++q)
+                    if (p.slot[q] >= 0)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) h[c][i] += w * y[i];
-                }
+                        for (int c = 0; c < NC; ++c) {
+                            const int col = (c * G + lane) * P;
+                            float y[P];
+                            load_elems<P>((const TH*)a.h + (int64_t)p.slot[q] * a.width + col, a.width - col, y);
+#pragma unroll
+                            for (int i = 0; i < P; ++i) h[c][i] += p.weight[q] * y[i];
+                        }
             }
         } else {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const int col = (c * G + lane) * 8;
-                load8((const TH*)a.h + row * a.width + col, a.width - col, h[c]);
+                const int col = (c * G + lane) * P;
+                load_elems<P>((const TH*)a.h + row * a.width + col, a.width - col, h[c]);
             }
         }
-        if (a.post_weight) normalise<G, NC>(h, a.post_weight, a.post_bias, a, lane, part, turn);
-        const int64_t gate_row = a.gate ? (row / a.rows_per_gate) * a.width : 0;
+        if (a.post_weight) {
+            if (!AHEAD) load_params<G, NC, P>(post, a.post_weight, a.post_bias, a, lane);
+            normalise<G, NC, P>(h, post, a, lane, part, turn);
+        }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = (c * G + lane) * 8;
+            const int col = (c * G + lane) * P;
             if (a.gate) {
-                float g[8];
-                if (a.gate_f32) load8((const float*)a.gate + gate_row + col, a.width - col, g);
-                else load8((const TH*)a.gate + gate_row + col, a.width - col, g);
+                if (!AHEAD) load_gate(c);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) h[c][i] *= gate_value(g[i], a.gate_act);
+                for (int i = 0; i < P; ++i) h[c][i] *= gate_value(gate[c][i], a.gate_act);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (col + i < a.width) x[c][i] += a.scale * h[c][i];
-            store8((TX*)a.x_out + row * a.width + col, a.width - col, x[c]);
+            for (int i = 0; i < P; ++i) x[c][i] += a.scale * h[c][i];            // zeros behind the row, like its weights
+            store_elems<P>((TX*)a.x_out + row * a.width + col, a.width - col, x[c]);
         }
     }
     if (a.pre_weight) {
-        normalise<G, NC>(x, a.pre_weight, a.pre_bias, a, lane, part, turn);
+        if (!AHEAD) load_params<G, NC, P>(pre, a.pre_weight, a.pre_bias, a, lane);
+        normalise<G, NC, P>(x, pre, a, lane, part, turn);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = (c * G + lane) * 8;
-            store8((TH*)a.u + row * a.width + col, a.width - col, x[c]);
+            const int col = (c * G + lane) * P;
+            store_elems<P>((TH*)a.u + row * a.width + col, a.width - col, x[c]);
         }
     }
 }
 
 template <typename TX, typename TH>
 static int launch_residual_norm(const NormArgs& a, hipStream_t stream) {
-    // Lanes per row: the fewest that hold it in at most 4 pieces a lane.  Wide rows, and rows of more than 512
-    // elements when there are too few to give every CU eight waves, take a whole workgroup.
-    const bool few = a.rows < 2048 && a.width > 512;
-#define FD_NORM(G, NC)                                                                                                \
+    // Lanes per row: 8 elements a lane up to 512 and in a workgroup's reach of 2048 (6000 rows of 2048 in bfloat16 with two
+    // choices: 32.1 us; a wave a row 42.9 us), but a wave for up to 1024 (8160 rows, float32 x: 26.2 us, a workgroup 37.7 us)
+    // unless there are too few rows to give every CU eight waves.
+    const bool few = a.rows < 2048;
+#define FD_NORM(G, NE)                                                                                                \
     do {                                                                                                              \
         const int64_t blocks = (a.rows + 256 / G - 1) / (256 / G);                                                    \
-        hipLaunchKernelGGL((residual_norm_kernel<TX, TH, G, NC>), dim3((unsigned)blocks), dim3(256), 0, stream, a);   \
+        hipLaunchKernelGGL((residual_norm_kernel<TX, TH, G, NE>), dim3((unsigned)blocks), dim3(256), 0, stream, a);   \
     } while (0)
-    if (a.width <= 128) FD_NORM(16, 1);
-    else if (a.width <= 512) FD_NORM(64, 1);
-    else if (few && a.width <= 2048) FD_NORM(256, 1);
-    else if (a.width <= 1024) FD_NORM(64, 2);
-    else if (a.width <= 2048) FD_NORM(64, 4);
-    else if (a.width <= 4096) FD_NORM(256, 2);
-    else if (a.width <= 8192) FD_NORM(256, 4);
-    else FD_NORM(256, 8);
+    if (a.width <= 128) FD_NORM(16, 8);
+    else if (a.width <= 512) FD_NORM(64, 8);
+    else if (a.width <= 1024 && !few) FD_NORM(64, 16);
+    else if (a.width <= 2048) FD_NORM(256, 8);
+    else if (a.width <= 4096) FD_NORM(256, 16);
+    else if (a.width <= 8192) FD_NORM(256, 32);
+    else FD_NORM(256, 64);
 #undef FD_NORM
     FD_LAUNCH_CHECK();
     return FD_OK;
@@ -177,14 +240,17 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const T* y, int64_t
     if (row >= rows) return;
     for (int col = (blockIdx.y * blockDim.x + threadIdx.x) * 8; col < width; col += gridDim.y * blockDim.x * 8) {
         float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int j = 0; j < k; ++j) {
-            const int32_t s = slots[row * k + j];
-            if (s < 0 || s >= y_rows) continue;
-            const float w = weights[row * k + j];
-            float v[8];
-            load8(y + (int64_t)s * width + col, width - col, v);
+        for (int j = 0; j < k; j += 2) {
+            const ChoicePair p = choice_pair(slots + row * k, weights + row * k, k, j, y_rows);
+            float v[2][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += w * v[i];
+            for (int q = 0; q < 2; ++q)
+                if (p.slot[q] >= 0) load8(y + (int64_t)p.slot[q] * width + col, width - col, v[q]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                if (p.slot[q] >= 0)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) acc[i] += p.weight[q] * v[q][i];
         }
         store8(out + row * width + col, width - col, acc);
     }

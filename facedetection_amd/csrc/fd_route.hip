@@ -5,19 +5,20 @@
 //   weights[t,j] = exp(l_j - l_0) / sum, the sum over the row's choices (normalize) or over all its experts
 //   slots[t,j]   = position of the choice among all choices sorted by (expert, t);  rows[slots[t,j]] = t
 //
-// Bound by the read of the logits.  A thread owns a row: it walks the row through LDS (staged by coalesced loads, 33
-// words a row so that the walk has no bank conflicts) and keeps its k best in registers, which takes 64 rows a wave
-// where a wave-wide arg-max would take 6 cross-lane steps a choice for one row.  A row's experts are distinct, so
+// Bound by the read of the logits, with the walk close behind it.  Two threads share a row: each walks its half of every 32
+// experts through LDS (staged by coalesced loads, 33 words a row so that the walk has no bank conflicts) and keeps its k
+// best in registers, which takes 32 rows a wave where a wave-wide arg-max would take 6 cross-lane steps a choice for one
+// row; the first thread then takes the other's in.  A row's experts are distinct, so
 // the rank of a choice among its workgroup's choices of that expert is a population count over one bit per row:
 // set with LDS atomics, whose order does not show.  Workgroups are joined by a second launch that sums their counts.
 #include "fd_elem.h"
 
 namespace fd {
 
-constexpr int ROUTE_ROWS = 512;            // rows and threads of a workgroup
+constexpr int ROUTE_ROWS = 512;            // rows of a workgroup; two threads a row choose, one places
 constexpr int ROUTE_COLS = 32;             // experts staged at a time
 constexpr int ROUTE_WORDS = ROUTE_ROWS / 64;
-constexpr int ROUTE_STAGE = ROUTE_ROWS * (ROUTE_COLS + 1);
+constexpr int ROUTE_STAGE = ROUTE_ROWS * (ROUTE_COLS + 2);   // rows of 33 words; later 2 words a choice and 2 more of a row
 
 struct RouteArgs {
     const void* logits;
@@ -27,7 +28,7 @@ struct RouteArgs {
     int32_t *chosen, *slots, *offsets, *source, *counts;     // counts [blocks, experts]: the workspace
 };
 
-// Exclusive scan of `v` over the workgroup's threads, in `words` (8 ints of LDS).  `all`: the sum.
+// Exclusive scan of `v` over the workgroup's first 512 threads, in `words` (an int of LDS a wave).  `all`: the sum.
 __device__ __forceinline__ int exclusive_scan(int v, int* words, int& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int sum = v;
@@ -48,20 +49,14 @@ __device__ __forceinline__ int exclusive_scan(int v, int* words, int& all) {
     return before + sum - v;
 }
 
-// exp(d) for d <= 0 by the hardware's exp2; what d * log2(e) lost in its rounding is put back to first order
-__device__ __forceinline__ float exp_below(float d) {
-    const float t = d * 1.44269504088896341f, lost = fmaf(d, 1.44269504088896341f, -t);
-    const float e = __builtin_amdgcn_exp2f(t);
-    return e > 0.f ? fmaf(e, lost * 0.693147180559945309f, e) : 0.f;          // d = -inf: lost is not a number
-}
-
 template <typename T, int KM>
-__global__ __launch_bounds__(ROUTE_ROWS) void expert_choose_kernel(RouteArgs a) {
+__global__ __launch_bounds__(2 * ROUTE_ROWS) void expert_choose_kernel(RouteArgs a) {
+    constexpr int HALF = ROUTE_COLS / 2;
     __shared__ float stage[ROUTE_STAGE];
     extern __shared__ unsigned long long bits[];                // [experts][ROUTE_WORDS]
-    const int t = threadIdx.x, row0 = blockIdx.x * ROUTE_ROWS, row = row0 + t;
+    const int tid = threadIdx.x, half = tid / ROUTE_ROWS, t = tid % ROUTE_ROWS, row0 = blockIdx.x * ROUTE_ROWS, row = row0 + t;
     const bool live = row < a.rows && (!a.mask || a.mask[row] != 0);
-    for (int i = t; i < a.experts * ROUTE_WORDS; i += ROUTE_ROWS) bits[i] = 0;
+    for (int i = tid; i < a.experts * ROUTE_WORDS; i += 2 * ROUTE_ROWS) bits[i] = 0;
 
     float top[KM];
     int best[KM];
@@ -70,53 +65,94 @@ __global__ __launch_bounds__(ROUTE_ROWS) void expert_choose_kernel(RouteArgs a) 
         top[i] = -INFINITY;
         best[i] = -1;
     }
-    float sum = 0.f, sum_at = -INFINITY;           // of exp(v - sum_at) over the row so far
-    // A thread fetches 8 experts of 4 rows, 4 threads a row; the next experts are on their way while these are walked.
-    float next[4][8];
+    float sum = 0.f, sum_at = -INFINITY;           // of exp(v - sum_at) over what the thread has seen
+    // A thread fetches 8 experts of 2 rows, 4 threads a row; the next experts are on their way while these are walked.
+    float next[2][8];
     auto fetch = [&](int c0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = (t >> 2) + i * (ROUTE_ROWS / 4), c = c0 + (t & 3) * 8;
+        for (int i = 0; i < 2; ++i) {
+            const int r = (tid >> 2) + i * (ROUTE_ROWS / 2), c = c0 + (tid & 3) * 8;
             load8((const T*)a.logits + (int64_t)(row0 + r) * a.experts + c, row0 + r < a.rows ? a.experts - c : 0, next[i]);
         }
     };
     fetch(0);
     for (int c0 = 0; c0 < a.experts; c0 += ROUTE_COLS) {
-        const int cols = min(ROUTE_COLS, a.experts - c0);
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) stage[((t >> 2) + i * (ROUTE_ROWS / 4)) * (ROUTE_COLS + 1) + (t & 3) * 8 + j] = next[i][j];
+            for (int j = 0; j < 8; ++j) stage[((tid >> 2) + i * (ROUTE_ROWS / 2)) * (ROUTE_COLS + 1) + (tid & 3) * 8 + j] = next[i][j];
         __syncthreads();
         if (c0 + ROUTE_COLS < a.experts) fetch(c0 + ROUTE_COLS);
-        if (live) {
-            const float* mine = stage + t * (ROUTE_COLS + 1);
+        const int first = c0 + half * HALF, cols = min(HALF, a.experts - first);
+        if (live && cols > 0) {
+            const float* mine = stage + t * (ROUTE_COLS + 1) + half * HALF;
 #pragma unroll 4
             for (int c = 0; c < cols; ++c) {
                 // sorted insert: an entry becomes the middle one of itself, the one above and v; equal values stay in front
-                const float raw = mine[c], v = raw > -INFINITY ? raw : -INFINITY;
+                const float v = fmaxf(mine[c], -INFINITY);          // not a number: the smallest
                 bool here[KM];
 #pragma unroll
                 for (int i = 0; i < KM; ++i) here[i] = v > top[i];
 #pragma unroll
                 for (int i = KM - 1; i > 0; --i) {
                     top[i] = __builtin_amdgcn_fmed3f(top[i - 1], top[i], v);
-                    best[i] = here[i - 1] ? best[i - 1] : (here[i] ? c0 + c : best[i]);
+                    best[i] = here[i - 1] ? best[i - 1] : (here[i] ? first + c : best[i]);
                 }
                 top[0] = fmaxf(top[0], v);
-                best[0] = here[0] ? c0 + c : best[0];
+                best[0] = here[0] ? first + c : best[0];
             }
             if (!a.normalize && top[0] > -INFINITY) {
-                if (sum_at != top[0]) sum = sum_at == -INFINITY ? 0.f : sum * expf(sum_at - top[0]);
+                if (sum_at != top[0]) sum = sum_at == -INFINITY ? 0.f : sum * exp_fast(sum_at - top[0]);
                 sum_at = top[0];
+                if (sum_at < INFINITY) {
 #pragma unroll 4
-                for (int c = 0; c < cols; ++c) {
-                    const float v = mine[c];
-                    sum += v == sum_at ? 1.f : (v < sum_at ? exp_below(v - sum_at) : 0.f);
+                    // exp2 without exp_fast's second term: its relative error grows with the distance that makes the value small
+                    for (int c = 0; c < cols; ++c) sum += __builtin_amdgcn_exp2f((fmaxf(mine[c], -INFINITY) - sum_at) * 1.44269504088896341f);
+                } else {
+                    for (int c = 0; c < cols; ++c) sum += mine[c] == INFINITY ? 1.f : 0.f;
                 }
             }
         }
+    }
+
+    // the second thread's choices and sum go to the first
+    __syncthreads();
+    float* his = stage + t;
+    if (half == 1) {
+#pragma unroll
+        for (int i = 0; i < KM; ++i) {
+            his[2 * i * ROUTE_ROWS] = top[i];
+            his[(2 * i + 1) * ROUTE_ROWS] = __int_as_float(best[i]);
+        }
+        his[2 * KM * ROUTE_ROWS] = sum;
+        his[(2 * KM + 1) * ROUTE_ROWS] = sum_at;
+    }
+    __syncthreads();
+    if (half == 0) {
+        const float other = his[2 * KM * ROUTE_ROWS], other_at = his[(2 * KM + 1) * ROUTE_ROWS], at = fmaxf(sum_at, other_at);
+        if (at > -INFINITY)
+            sum = (sum_at == at ? sum : (sum_at == -INFINITY ? 0.f : sum * exp_fast(sum_at - at))) +
+                  (other_at == at ? other : (other_at == -INFINITY ? 0.f : other * exp_fast(other_at - at)));
+#pragma unroll
+        for (int q = 0; q < KM; ++q) {
+            const float v = his[2 * q * ROUTE_ROWS];
+            const int x = __float_as_int(his[(2 * q + 1) * ROUTE_ROWS]);
+            if (x < 0) break;
+            bool here[KM];
+#pragma unroll
+            for (int i = 0; i < KM; ++i) here[i] = v > top[i] || (v == top[i] && x < best[i]);
+#pragma unroll
+            for (int i = KM - 1; i > 0; --i) {
+                top[i] = here[i - 1] ? top[i - 1] : (here[i] ? v : top[i]);
+                best[i] = here[i - 1] ? best[i - 1] : (here[i] ? x : best[i]);
+            }
+            top[0] = here[0] ? v : top[0];
+            best[0] = here[0] ? x : best[0];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < KM; ++i) best[i] = -1;
     }
 
     float e[KM];
@@ -136,19 +172,22 @@ __global__ __launch_bounds__(ROUTE_ROWS) void expert_choose_kernel(RouteArgs a) 
     if (t < a.experts)
 #pragma unroll
         for (int w = 0; w < ROUTE_WORDS; ++w) n += __popcll(bits[t * ROUTE_WORDS + w]);
+    static_assert(2 * FD_ROUTE_MAX_K + 2 <= ROUTE_COLS + 2, "what the second thread hands over fits the stage");
     int* base = (int*)stage;
     if (a.blocks == 1) {
         int all;
         const int first = exclusive_scan(n, base + ROUTE_ROWS, all);
-        base[t] = first;
-        if (t < a.experts) a.offsets[t] = first;
-        if (t == 0) a.offsets[a.experts] = all;
+        if (half == 0) {
+            base[t] = first;
+            if (t < a.experts) a.offsets[t] = first;
+            if (t == 0) a.offsets[a.experts] = all;
+        }
         __syncthreads();
-        for (int i = all + t; i < a.rows * a.k; i += ROUTE_ROWS) a.source[i] = -1;
-    } else if (t < a.experts) {
+        for (int i = all + tid; i < a.rows * a.k; i += 2 * ROUTE_ROWS) a.source[i] = -1;
+    } else if (half == 0 && t < a.experts) {
         a.counts[(int64_t)blockIdx.x * a.experts + t] = n;
     }
-    if (row >= a.rows) return;
+    if (half == 1 || row >= a.rows) return;
 #pragma unroll
     for (int i = 0; i < KM; ++i) {
         if (i >= a.k) continue;
@@ -229,7 +268,7 @@ __global__ __launch_bounds__(ROUTE_ROWS) void expert_place_kernel(RouteArgs a) {
 
 template <typename T>
 static void launch_choose(const RouteArgs& a, hipStream_t s) {
-    const dim3 grid(a.blocks), block(ROUTE_ROWS);
+    const dim3 grid(a.blocks), block(2 * ROUTE_ROWS);
     const size_t lds = (size_t)a.experts * ROUTE_WORDS * sizeof(unsigned long long);
     if (a.k == 1) hipLaunchKernelGGL((expert_choose_kernel<T, 1>), grid, block, lds, s, a);
     else if (a.k == 2) hipLaunchKernelGGL((expert_choose_kernel<T, 2>), grid, block, lds, s, a);
