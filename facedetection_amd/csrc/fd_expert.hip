@@ -550,7 +550,8 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void expert_dma_kernel(ExpertArg
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// 256 x 256 tiles, 16-bit types, one workgroup of 2 x 4 waves a CU.  A wave's 128 x 64 sums fill 128 accumulation registers; the
+// Large tiles, 16-bit types: 32 MI x 256 (MI = 8: 256 x 256), one workgroup of 2 x 4 waves a CU.  A wave's 128 x 64 sums fill 128
+// accumulation registers; the
 // products of a 64-byte half step of a CU are 1024 cycles of its matrix units, its fragment reads 768 and the loads into
 // LDS 256 cycles of LDS, so everything that is not a product has to run beside the products: that is what the order below
 // is for.  Measured on 32768 rows x 2048 x 4096: 1.17 PFLOP/s from memory and 1.34 when all rows lie in L2, where the large
@@ -576,12 +577,12 @@ __device__ __forceinline__ void settle(f32x4_t (&acc)[4]) {
     asm volatile("s_nop 15\ns_nop 15" : "+a"(acc[0]), "+a"(acc[1]), "+a"(acc[2]), "+a"(acc[3])::"memory");
 }
 
-// The results of a wave of the 256 x 256 tile (128 rows from m0 on, weight rows wn .. wn + 63): bias, activation, gate and
+// The results of a wave of the large tile (16 MI rows from m0 on, weight rows wn .. wn + 63): bias, activation, gate and
 // rounding in registers, 16 rows at a time through the wave's 2 KB of LDS to 16-byte stores (N is a multiple of 8).
 // The loads of the next tile's first two steps are awaited before the first store, so that no later wait for loads is
 // one for stores.
-template <typename T, int ACT, bool GATED>
-__device__ __forceinline__ void store_wide(const ExpertArgs& a, int e, int m0, int m1, int n0, int wn, const f32x4_t (&acc)[8][4], char* part) {
+template <typename T, int ACT, bool GATED, int MI>
+__device__ __forceinline__ void store_wide(const ExpertArgs& a, int e, int m0, int m1, int n0, int wn, const f32x4_t (&acc)[MI][4], char* part) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     const int lane = opaque(threadIdx.x & 63), quad = lane >> 4, r = lane & 15;
     const int first = n0 + (GATED ? wn / 2 : wn);                   // output column of the wave
@@ -604,7 +605,7 @@ __device__ __forceinline__ void store_wide(const ExpertArgs& a, int e, int m0, i
     const int row0 = lane / PIECES, p = lane % PIECES, n = first + p * 8;
     T* out = (T*)a.y + (int64_t)(m0 + row0) * a.N + n;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < MI; ++j) {
 #pragma unroll
         for (int i = 0; i < 4; i += GATED ? 2 : 1) {
             T4 q;
@@ -627,14 +628,14 @@ __device__ __forceinline__ void store_wide(const ExpertArgs& a, int e, int m0, i
     }
 }
 
-template <typename T, int ACT, bool GATED>
+template <typename T, int ACT, bool GATED, int MI>
 __global__ __launch_bounds__(512, 2) void expert_wide_kernel(ExpertArgs a, unsigned x_bytes) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int BM = 256, BN = 256, WN = 4, WAVES = 8, G = BM / 8 / WAVES, STAGE = (BM + BN) * 128;
-    constexpr int MI = 8, NI = 4, EARLY = 1;
+    constexpr int BM = 32 * MI, ROWS = 256, BN = 256, WN = 4, WAVES = 8, G = ROWS / 8 / WAVES, STAGE = (ROWS + BN) * 128;
+    constexpr int NI = 4, EARLY = 1;
     constexpr unsigned NONE = 0x80000000u;
     // one array: the compiler waits for all loads into LDS before it reads an array of its own
-    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + WAVES * 2048 + (FD_EXPERT_MAX + BM) * 4];
+    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + WAVES * 2048 + (FD_EXPERT_MAX + ROWS) * 4];
     int *ends = (int*)(smem + 2 * STAGE + WAVES * 2048), *list = ends + FD_EXPERT_MAX;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const TileScan scan = scan_tiles(a, BM, ends);
@@ -654,7 +655,7 @@ __global__ __launch_bounds__(512, 2) void expert_wide_kernel(ExpertArgs a, unsig
         Tile t;
         locate_tile(scan, a, ends, BM, tile / a.tiles_n, t.e, t.m0, t.m1);
         t.n0 = (tile % a.tiles_n) * (a.gated ? BN / 2 : BN);
-        if (a.rows && wave < BM / 64) {
+        if (a.rows && wave < ROWS / 64) {
             const __amdgpu_buffer_rsrc_t lr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.rows + t.m0), 0, (unsigned)(t.m1 - t.m0) * 4, 0x00020000);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(lr, (__attribute__((address_space(3))) void*)(list + wave * 64), 4, (wave * 64 + opaque(lane)) * 4, 0, 0, 0);
         }
@@ -662,7 +663,7 @@ __global__ __launch_bounds__(512, 2) void expert_wide_kernel(ExpertArgs a, unsig
     };
     unsigned xo[G], wo[G];                      // byte offset of the lane's piece of step 0, NONE for no row
     auto address = [&](const Tile& t) {
-        const int64_t limit = a.rows ? a.x_rows : BM;
+        const int64_t limit = a.rows ? a.x_rows : ROWS;
         const int lrow = wave * 8 + (opaque(lane) >> 3);
 #pragma unroll
         for (int i = 0; i < G; ++i) {
@@ -687,21 +688,21 @@ __global__ __launch_bounds__(512, 2) void expert_wide_kernel(ExpertArgs a, unsig
             __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void*)(base + WAVES * i * 1024), 16,
                                                      none ? NONE : xo[i % G], step * 128, 0, 0);
         else
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void*)(base + BM * 128 + WAVES * (i - G) * 1024), 16,
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void*)(base + ROWS * 128 + WAVES * (i - G) * 1024), 16,
                                                      none ? NONE : wo[i % G], step * 128, 0, 0);
     };
     auto issue = [&](int step, int stage) {
 #pragma unroll
         for (int i = 0; i < 2 * G; ++i) load(i, step, stage);
     };
-    const int wm = (wave / WN) * 128, wn = (wave % WN) * 64;
+    const int wm = (wave / WN) * (BM / 2), wn = (wave % WN) * 64;
     const int frow = lane & 15, sw = (frow >> 1) & 7;
     int xf_off[2], wf_off[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int pos = ((h * 4 + (lane >> 4)) ^ sw) * 16;
         xf_off[h] = (wm + frow) * 128 + pos;
-        wf_off[h] = (BM + wn + frow) * 128 + pos;
+        wf_off[h] = (ROWS + wn + frow) * 128 + pos;
     }
 
     // One pipeline over all steps of all tiles.  Fragments are read half a step ahead: a row fragment is replaced by that
@@ -778,7 +779,7 @@ __global__ __launch_bounds__(512, 2) void expert_wide_kernel(ExpertArgs a, unsig
         run(std::integral_constant<int, 2>(), steps - 1, nxt, acc);
 #pragma unroll
         for (int j = 0; j < MI; ++j) settle(acc[j]);
-        store_wide<T, ACT, GATED>(a, cur.e, cur.m0 + wm, cur.m1, cur.n0, wn, acc, smem + 2 * STAGE + wave * 2048);
+        store_wide<T, ACT, GATED, MI>(a, cur.e, cur.m0 + wm, cur.m1, cur.n0, wn, acc, smem + 2 * STAGE + wave * 2048);
         cur = nxt;
     }
     wait_vmcnt<0>();
@@ -925,26 +926,26 @@ static int launch_expert_dma(ExpertArgs a, hipStream_t stream) {
     return FD_OK;
 }
 
-template <typename T, int ACT>
+template <typename T, int MI, int ACT>
 static int launch_expert_wide(ExpertArgs a, hipStream_t stream) {
     a.tiles_n = ceil_div(a.N, a.gated ? 128 : 256);
-    const int grid = tile_grid(a, 256, 1);
+    const int grid = tile_grid(a, 32 * MI, 1);
     if (!grid) return FD_ERR_LIMIT;
     const unsigned x_bytes = (unsigned)(a.x_rows * a.K * (int64_t)sizeof(T));
     ProfScope scope(stream, "expert_wide", expert_flops(a), expert_bytes<T>(a));
-    if (a.gated) hipLaunchKernelGGL((expert_wide_kernel<T, ACT, true>), dim3(grid), dim3(512), 0, stream, a, x_bytes);
-    else hipLaunchKernelGGL((expert_wide_kernel<T, ACT, false>), dim3(grid), dim3(512), 0, stream, a, x_bytes);
+    if (a.gated) hipLaunchKernelGGL((expert_wide_kernel<T, ACT, true, MI>), dim3(grid), dim3(512), 0, stream, a, x_bytes);
+    else hipLaunchKernelGGL((expert_wide_kernel<T, ACT, false, MI>), dim3(grid), dim3(512), 0, stream, a, x_bytes);
     FD_LAUNCH_CHECK();
     return FD_OK;
 }
 
-template <typename T>
+template <typename T, int MI>
 static int launch_expert_wide(const ExpertArgs& a, hipStream_t stream) {
     switch (a.act) {
-        case FD_ACT_RELU: return launch_expert_wide<T, FD_ACT_RELU>(a, stream);
-        case FD_ACT_SILU: return launch_expert_wide<T, FD_ACT_SILU>(a, stream);
-        case FD_ACT_GELU: return launch_expert_wide<T, FD_ACT_GELU>(a, stream);
-        default: return launch_expert_wide<T, FD_ACT_NONE>(a, stream);
+        case FD_ACT_RELU: return launch_expert_wide<T, MI, FD_ACT_RELU>(a, stream);
+        case FD_ACT_SILU: return launch_expert_wide<T, MI, FD_ACT_SILU>(a, stream);
+        case FD_ACT_GELU: return launch_expert_wide<T, MI, FD_ACT_GELU>(a, stream);
+        default: return launch_expert_wide<T, MI, FD_ACT_NONE>(a, stream);
     }
 }
 
@@ -975,10 +976,12 @@ static bool dma_rows(const ExpertArgs& a) {
 // workgroup (float32, the 20 slots: 31.9 us, with four 34.8 us).
 //
 // Otherwise tiles.  A CU works through ceil(tiles / CUs) of them, and one step of 128 bytes of K costs a CU (with all CUs
-// busy) 1.75 us for 256 x 256, 0.57 us for 128 x 128, 0.37 us for 64 x 128 and 0.27 us for 64 x 64; a 256 x 256 tile, alone
-// on its CU, another 4.5 us for its ends.  Large tiles win on many rows an expert (32768 rows, 2048 x 4096: 1.17 PFLOP/s
-// against 0.94, 0.73 and 0.51), small ones when an expert has few or the last round of tiles is nearly empty (1200 slots on
-// 16 experts of 2 x 1024 x 1024: 33, 22, 20 and 20 us).  The largest takes outputs in eights and three steps or more.
+// busy) 1.75, 1.48 and 1.34 us for 256, 224 and 192 x 256, 0.57 us for 128 x 128, 0.37 us for 64 x 128 and 0.27 us for 64 x 64;
+// the large ones, alone on their CU, another 3.5 to 4 us for their ends.  Large tiles win on many rows an expert (32768 rows,
+// 2048 x 4096: 1.22 PFLOP/s for 256 x 256, 0.93, 0.73 and 0.51 for the small ones), a little smaller ones when the last round
+// of tiles is nearly empty (12000 slots on 8 experts of 2048 x 2048: 126 us with 256 rows, 113 with 224, 133 with 192; 8000 on
+// 32 experts of 2 x 1024 x 1024: 71, 64, 60 us), small ones when an expert has few (1200 slots on 16 such experts: 29 us with
+// 256 x 256, 21, 20 and 20 us).  The large ones take outputs in eights and three steps or more.
 // Through registers, for rows that are not aligned, it is 1.07 us for 128 x 128 and 0.41 us for 64 x 64 (62682 slots,
 // 1448 x 1001: 394 and 583 us; 2331 slots, 333 x 1001: 34 and 17 us).  In float32 the matrix units are slow enough (1/16)
 // that every tile reaches the same rate (126 TFLOP/s) and the smallest wastes the least.
@@ -1000,11 +1003,21 @@ static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
     if constexpr (sizeof(T) == 4) {
         return launch_expert_dma<T, 64, 64, 2, 2, 4>(a, stream);
     } else {
-        const double c256 = cost(256, 256, 1.75, 4.5), c128 = cost(128, 128, 0.57, 1.0), c64x128 = cost(64, 128, 0.37, 0.5), c64 = cost(64, 64, 0.27, 0.3);
-        if (a.N % 8 == 0 && row_bytes > 256 && c256 <= c128 && c256 <= c64x128 && c256 <= c64) return launch_expert_wide<T>(a, stream);
-        if (c128 <= c64x128 && c128 <= c64) return launch_expert_dma<T, 128, 128, 2, 2, 2>(a, stream);
-        if (c64x128 <= c64) return launch_expert_dma<T, 64, 128, 2, 2, 3>(a, stream);
-        return launch_expert_dma<T, 64, 64, 2, 2, 4>(a, stream);
+        struct {
+            double cost;
+            int (*launch)(const ExpertArgs&, hipStream_t);
+        } tiles[] = {
+            {cost(256, 256, 1.75, 3.9), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 8>(p, q); }},
+            {cost(224, 256, 1.48, 3.6), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 7>(p, q); }},
+            {cost(192, 256, 1.34, 3.4), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 6>(p, q); }},
+            {cost(128, 128, 0.57, 1.0), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 128, 128, 2, 2, 2>(p, q); }},
+            {cost(64, 128, 0.37, 0.5), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 128, 2, 2, 3>(p, q); }},
+            {cost(64, 64, 0.27, 0.3), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 64, 2, 2, 4>(p, q); }},
+        };
+        int best = a.N % 8 == 0 && row_bytes > 256 ? 0 : 3;
+        for (int i = best + 1; i < 6; ++i)
+            if (tiles[i].cost < tiles[best].cost) best = i;
+        return tiles[best].launch(a, stream);
     }
 }
 
