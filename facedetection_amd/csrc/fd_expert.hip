@@ -983,7 +983,8 @@ static bool dma_rows(const ExpertArgs& a) {
 // 32 experts of 2 x 1024 x 1024: 71, 64, 60 us), small ones when an expert has few (1200 slots on 16 such experts: 29 us with
 // 256 x 256, 21, 20 and 20 us).  The large ones take outputs in eights and three steps or more.
 // Through registers, for rows that are not aligned, it is 1.07 us for 128 x 128 and 0.41 us for 64 x 64 (62682 slots,
-// 1448 x 1001: 394 and 583 us; 2331 slots, 333 x 1001: 34 and 17 us).  In float32 the matrix units are slow enough (1/16)
+// 1448 x 1001: 394 and 583 us; 2331 slots, 333 x 1001: 34 and 17 us), and with less than a 64 x 64 tile a CU 32 x 64 spreads
+// the loads (400 slots, 733 x 1001: 12.2 us, 14.5 with 64 x 64).  In float32 the matrix units are slow enough (1/16)
 // that every tile reaches the same rate (126 TFLOP/s) and the smallest wastes the least.
 template <typename T>
 static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
@@ -993,10 +994,12 @@ static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
     if (a.slots <= 32 || a.slots <= 24 * groups) return launch_expert_stream<T, 2, 4, 4>(a, stream);
     const int steps = ceil_div(row_bytes, 128);
     auto cost = [&](int bm, int bn, double step, double ends) {
-        const double tiles = (a.slots / (double)bm + groups / 2.0) * ceil_div(a.wrows, bn);
-        return ceil_div((int64_t)tiles + 1, compute_units()) * (steps * step + ends);
+        // a group ends in half a tile on average, a single one where it does
+        const double rows = groups == 1 ? ceil_div(a.slots, bm) : a.slots / (double)bm + groups / 2.0;
+        return ceil(rows * ceil_div(a.wrows, bn) / compute_units()) * (steps * step + ends);
     };
     if (!dma_rows<T>(a)) {
+        if (cost(64, 64, 1.0, 0.0) <= steps) return launch_expert_tile<T, 32, 64, 2, 4>(a, stream);
         if (sizeof(T) == 4 || cost(64, 64, 0.41, 0.3) <= cost(128, 128, 1.07, 1.0)) return launch_expert_tile<T, 64, 64, 2, 4>(a, stream);
         return launch_expert_tile<T, 128, 128, 1, 2>(a, stream);
     }

@@ -223,6 +223,8 @@ def _rows(a, index, name, dtype=None):
 
 
 def _typed(a, index, name, dtype=None):
+    if isinstance(a, torch.Tensor) and a.dtype is dtype:
+        return runtime.rows_to_device(a, dtype, index)
     t = _row_type(a)
     if dtype is not None and t != dtype:
         if (a.dtype if isinstance(a, torch.Tensor) else _NP_TYPES.get(a.dtype.name)) in _DTYPES:
@@ -233,7 +235,7 @@ def _typed(a, index, name, dtype=None):
 
 def _ints(a, index, name):
     """int32 indices on the GPU; a wider type is refused, since a conversion could wrap."""
-    if str(a.dtype).split(".")[-1] != "int32":
+    if a.dtype is not torch.int32 and str(a.dtype) != "int32":
         raise ValueError("%s must be int32, not %s" % (name, a.dtype))
     return runtime.rows_to_device(a, torch.int32, index)
 

@@ -100,7 +100,7 @@ def current():
 def rows_to_device(array, dtype, index):
     """Contiguous tensor of ``dtype`` on GPU ``index``; one that is both already is returned as it is."""
     if isinstance(array, torch.Tensor):
-        if array.dtype == dtype and array.is_cuda and array.get_device() == index and array.is_contiguous():
+        if array.dtype is dtype and array.get_device() == index and array.is_contiguous():      # the host is device -1
             return array
         return array.to(device="cuda:%d" % index, dtype=dtype).contiguous()
     return torch.from_numpy(np.ascontiguousarray(array)).to(device="cuda:%d" % index, dtype=dtype)
