@@ -207,6 +207,102 @@ __global__ __launch_bounds__(2 * ROUTE_ROWS) void expert_choose_kernel(RouteArgs
     }
 }
 
+// Largest value of a wave, and its sum, in every lane: shifts within rows of 16, then row 0 to 1 and 2 to 3, then the half.
+__device__ __forceinline__ float wave_max(float v) {
+#define FD_STEP(CTRL, ROWS) \
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, ROWS, 0xf, false)))
+    FD_STEP(0x111, 0xf); FD_STEP(0x112, 0xf); FD_STEP(0x114, 0xf); FD_STEP(0x118, 0xf); FD_STEP(0x142, 0xa); FD_STEP(0x143, 0xc);
+#undef FD_STEP
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#define FD_STEP(CTRL, ROWS) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false))
+    FD_STEP(0x111, 0xf); FD_STEP(0x112, 0xf); FD_STEP(0x114, 0xf); FD_STEP(0x118, 0xf); FD_STEP(0x142, 0xa); FD_STEP(0x143, 0xc);
+#undef FD_STEP
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// Up to FEW_ROWS rows, one workgroup: a wave takes a row, expert 64 i + l in lane l, and finds its choices one by one; the
+// walk of the other kernel would leave most lanes idle through every expert (5 rows of 145 experts, 8 choices: 6 us, the
+// walk 24; 64 rows of 200: 20 and 28 us; 128 rows of 64 experts, 4 choices: 15 and 9 us).
+constexpr int FEW_ROWS = 64;
+
+template <typename T, int VALUES>
+__global__ __launch_bounds__(2 * ROUTE_ROWS) void expert_choose_few_kernel(RouteArgs a) {
+    __shared__ unsigned long long bits[FD_ROUTE_MAX_EXPERTS];          // of an expert: a bit a row
+    __shared__ int best[FEW_ROWS * FD_ROUTE_MAX_K], base[ROUTE_ROWS], words[2 * ROUTE_WORDS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int i = tid; i < a.experts; i += 2 * ROUTE_ROWS) bits[i] = 0;
+    __syncthreads();
+    for (int row = wave; row < a.rows; row += 2 * ROUTE_WORDS) {
+        const bool live = !a.mask || a.mask[row] != 0;
+        float v[VALUES], all = 0.f;
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) {
+            const int x = 64 * i + lane;
+            v[i] = live && x < a.experts ? fmaxf((float)((const T*)a.logits)[(int64_t)row * a.experts + x], -INFINITY) : -INFINITY;
+        }
+        float first = -INFINITY, mine = 0.f, mine_sum = 0.f;        // lane j keeps exp(choice j - choice 0)
+        int mine_at = -1;
+        for (int j = 0; j < a.k; ++j) {
+            float m = v[0];
+#pragma unroll
+            for (int i = 1; i < VALUES; ++i) m = fmaxf(m, v[i]);
+            m = wave_max(m);
+            if (m == -INFINITY) break;
+            if (j == 0) {
+                first = m;
+#pragma unroll
+                for (int i = 0; i < VALUES; ++i) all += v[i] == first ? 1.f : (v[i] > -INFINITY ? exp_fast(v[i] - first) : 0.f);
+            }
+            // the lowest expert that has it, which loses it
+            int at = -1;
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) {
+                const unsigned long long who = __ballot(v[i] == m);
+                if (at < 0 && who) {
+                    at = 64 * i + __ffsll(who) - 1;
+                    if (lane == (at & 63)) v[i] = -INFINITY;
+                }
+            }
+            const float e = m == first ? 1.f : exp_fast(m - first);
+            mine_sum += e;
+            if (lane == j) {
+                mine = e;
+                mine_at = at;
+            }
+            if (lane == 0) atomicOr(&bits[at], 1ull << row);
+        }
+        const float sum = a.normalize ? mine_sum : wave_sum(all);
+        if (lane < a.k) {
+            const int64_t i = (int64_t)row * a.k + lane;
+            a.weights[i] = mine_at >= 0 ? mine / sum : 0.f;
+            a.chosen[i] = mine_at;
+            best[i] = mine_at;
+        }
+    }
+    __syncthreads();
+    const int n = tid < a.experts ? __popcll(bits[tid]) : 0;
+    int all;
+    const int begin = exclusive_scan(n, words, all);
+    if (tid < ROUTE_ROWS) {
+        base[tid] = begin;
+        if (tid < a.experts) a.offsets[tid] = begin;
+    }
+    if (tid == 0) a.offsets[a.experts] = all;
+    __syncthreads();
+    for (int i = tid; i < a.rows * a.k; i += 2 * ROUTE_ROWS) {
+        const int row = i / a.k, x = best[i];
+        int at = -1;
+        if (x >= 0) {
+            at = base[x] + __popcll(bits[x] & ((1ull << row) - 1));
+            a.source[at] = row;
+        }
+        a.slots[i] = at;
+        if (i >= all) a.source[i] = -1;
+    }
+}
+
 // Adds to every choice's rank the choices of earlier experts and of earlier workgroups.
 __global__ __launch_bounds__(ROUTE_ROWS) void expert_place_kernel(RouteArgs a) {
     __shared__ int before[ROUTE_ROWS], total[ROUTE_ROWS], words[ROUTE_WORDS];
@@ -268,6 +364,12 @@ __global__ __launch_bounds__(ROUTE_ROWS) void expert_place_kernel(RouteArgs a) {
 
 template <typename T>
 static void launch_choose(const RouteArgs& a, hipStream_t s) {
+    if (a.rows <= FEW_ROWS) {
+        if (a.experts <= 64) hipLaunchKernelGGL((expert_choose_few_kernel<T, 1>), dim3(1), dim3(2 * ROUTE_ROWS), 0, s, a);
+        else if (a.experts <= 256) hipLaunchKernelGGL((expert_choose_few_kernel<T, 4>), dim3(1), dim3(2 * ROUTE_ROWS), 0, s, a);
+        else hipLaunchKernelGGL((expert_choose_few_kernel<T, 8>), dim3(1), dim3(2 * ROUTE_ROWS), 0, s, a);
+        return;
+    }
     const dim3 grid(a.blocks), block(2 * ROUTE_ROWS);
     const size_t lds = (size_t)a.experts * ROUTE_WORDS * sizeof(unsigned long long);
     if (a.k == 1) hipLaunchKernelGGL((expert_choose_kernel<T, 1>), grid, block, lds, s, a);

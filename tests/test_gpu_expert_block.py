@@ -78,7 +78,7 @@ def _check_route(logits, k, mask=None, normalize=True):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T,E,k,normalize,masked", [
     (1, 1, 1, True, False), (1, 5, 2, False, False), (10, 8, 2, True, False), (63, 33, 3, False, True), (512, 64, 4, True, True),
-    (513, 7, 7, True, False), (700, 200, 5, False, False), (1025, 512, 16, True, True), (2500, 31, 9, False, True), (64, 65, 8, True, False),
+    (513, 7, 7, True, False), (700, 200, 5, False, False), (1025, 512, 16, True, True), (2500, 31, 9, False, True), (64, 65, 8, True, False), (64, 300, 16, False, True), (65, 300, 16, False, True), (40, 64, 3, False, False),
 ])
 def test_route(dtype, T, E, k, normalize, masked):
     g = _gen(T * 1000 + E)
