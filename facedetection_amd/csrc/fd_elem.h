@@ -24,42 +24,41 @@ inline int with_dtype(int t, F&& f) {
     }
 }
 
-// P elements from p as float32; elements from `n` on are zero and not read
+// P elements from or to p; the one rounding to fewer bits is to nearest even, at the end of an operator
 template <int P, typename T>
-__device__ __forceinline__ void load_elems(const T* p, int n, float (&v)[P]) {
-    if (n >= P) {
-        T raw[P];
-        __builtin_memcpy(raw, p, sizeof(raw));
+__device__ __forceinline__ void load_whole(const T* p, float (&v)[P]) {
+    T raw[P];
+    __builtin_memcpy(raw, p, sizeof(raw));
 #pragma unroll
-        for (int i = 0; i < P; ++i) v[i] = (float)raw[i];
-    } else {
+    for (int i = 0; i < P; ++i) v[i] = (float)raw[i];
+}
+template <int P, typename T>
+__device__ __forceinline__ void store_whole(T* p, const float (&v)[P]) {
+    T raw[P];
 #pragma unroll
-        for (int i = 0; i < P; ++i) v[i] = i < n ? (float)p[i] : 0.f;
-    }
+    for (int i = 0; i < P; ++i) raw[i] = (T)v[i];
+    __builtin_memcpy(p, raw, sizeof(raw));
 }
 
-// the one rounding to fewer bits: to nearest even, at the end of the operator
-template <int P, typename T>
-__device__ __forceinline__ void store_elems(T* p, int n, const float (&v)[P]) {
-    if (n >= P) {
-        T raw[P];
-#pragma unroll
-        for (int i = 0; i < P; ++i) raw[i] = (T)v[i];
-        __builtin_memcpy(p, raw, sizeof(raw));
-    } else {
-#pragma unroll
-        for (int i = 0; i < P; ++i)
-            if (i < n) p[i] = (T)v[i];
-    }
-}
-
+// 8 elements as float32; elements from `n` on are zero and not read, or not written
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
-    load_elems<8>(p, n, v);
+    if (n >= 8) {
+        load_whole<8>(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+    }
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
-    store_elems<8>(p, n, v);
+    if (n >= 8) {
+        store_whole<8>(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = (T)v[i];
+    }
 }
 
 // exp(d) by the hardware's exp2; what d * log2(e) lost in its rounding is put back to first order

@@ -44,19 +44,56 @@ __device__ __forceinline__ float row_sum(float v, float (*part)[4], int& turn) {
     return v;
 }
 
+// The pieces of a lane: piece c has P elements from column at[c] on, and those before own[c] belong to another lane.  Pieces lie
+// G * P apart; one that would end behind the row (of P elements or more) is moved back to the row's last P.  It then
+// computes, and writes, the same values for the columns that it shares, and leaves them out of sums; whole pieces without a
+// branch keep all loads of a row on their way at once (with partial pieces read element by element: 101351 x 947 in
+// bfloat16 148 us).
+template <int NC>
+struct Pieces {
+    int at[NC], own[NC];
+    bool whole;                // every piece lies in the row
+};
+
+template <int G, int NC, int P>
+__device__ __forceinline__ Pieces<NC> row_pieces(int lane, int width) {
+    Pieces<NC> q;
+    q.whole = width == G * NC * P;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int col = (c * G + lane) * P;
+        q.at[c] = min(col, width - P);
+        q.own[c] = min(col - q.at[c], P);
+    }
+    return q;
+}
+
+template <int NC, int P>
+__device__ __forceinline__ float own_sum(const float (&v)[NC][P], const Pieces<NC>& q, bool square) {
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const float e = q.whole || i >= q.own[c] ? v[c][i] : 0.f;
+            s = square ? fmaf(e, e, s) : s + e;
+        }
+    return s;
+}
+
 // weight and bias of a lane's pieces
 template <int NC, int P>
 struct NormParams {
     float weight[NC][P], bias[NC][P];
 };
 
-template <int G, int NC, int P>
-__device__ __forceinline__ void load_params(NormParams<NC, P>& p, const float* weight, const float* bias, const NormArgs& a, int lane) {
+template <int NC, int P>
+__device__ __forceinline__ void load_params(NormParams<NC, P>& p, const float* weight, const float* bias, const Pieces<NC>& q) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) load_whole<P>(weight + q.at[c], p.weight[c]);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int col = (c * G + lane) * P;
-        load_elems<P>(weight + col, a.width - col, p.weight[c]);
-        if (bias) load_elems<P>(bias + col, a.width - col, p.bias[c]);
+        if (bias) load_whole<P>(bias + q.at[c], p.bias[c]);
         else
 #pragma unroll
             for (int i = 0; i < P; ++i) p.bias[c][i] = 0.f;
@@ -64,40 +101,23 @@ __device__ __forceinline__ void load_params(NormParams<NC, P>& p, const float* w
 }
 
 template <int G, int NC, int P>
-__device__ __forceinline__ void normalise(float (&v)[NC][P], const NormParams<NC, P>& p, const NormArgs& a, int lane, float (*part)[4], int& turn) {
+__device__ __forceinline__ void normalise(float (&v)[NC][P], const NormParams<NC, P>& p, const Pieces<NC>& q, const NormArgs& a, float (*part)[4],
+                                          int& turn) {
     if (a.layer) {
-        float s = 0.f;
+        const float mean = row_sum<G>(own_sum(v, q, false), part, turn) / (float)a.width;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int i = 0; i < P; ++i) s += v[c][i];
-        const float mean = row_sum<G>(s, part, turn) / (float)a.width;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int left = a.width - (c * G + lane) * P;         // elements behind the row stay zero
-            if (left >= P) {
-#pragma unroll
-                for (int i = 0; i < P; ++i) v[c][i] -= mean;
-            } else {
-#pragma unroll
-                for (int i = 0; i < P; ++i)
-                    if (i < left) v[c][i] -= mean;
-            }
-        }
+            for (int i = 0; i < P; ++i) v[c][i] -= mean;
     }
-    float s = 0.f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int i = 0; i < P; ++i) s += v[c][i] * v[c][i];
-    const float r = rsqrtf(row_sum<G>(s, part, turn) / (float)a.width + a.eps);
+    const float r = rsqrtf(row_sum<G>(own_sum(v, q, true), part, turn) / (float)a.width + a.eps);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int i = 0; i < P; ++i) v[c][i] = v[c][i] * r * p.weight[c][i] + p.bias[c][i];
 }
 
-// Two of a row's choices, so that both rows are on their way before either is added; -1 for a choice that is not made.
+// Two of a row's choices, so that both are asked for before either is waited for; -1 for a choice that is not made.
 struct ChoicePair {
     int32_t slot[2];
     float weight[2];
@@ -115,46 +135,39 @@ __device__ __forceinline__ ChoicePair choice_pair(const int32_t* slots, const fl
     return p;
 }
 
-// G lanes hold a row, NE elements each, in pieces of P: element (c * G + lane) * P + i.  A piece is 16 bytes of x, 4 elements
-// of a float32 x and 8 otherwise, so that neighbouring lanes read neighbouring pieces.  With 8 elements a lane there are
+// G lanes hold a row, NE elements each.  A piece is 16 bytes of x, 4 elements of a float32 x and 8 otherwise, so that neighbouring
+// lanes read neighbouring pieces; rows shorter than that are read one by one (P = 1).  With 8 elements a lane there are
 // registers to ask for everything that the row needs before the first sum is waited for.
-template <typename TX>
-__host__ __device__ constexpr int piece_elems() {
-    return 16 / (int)sizeof(TX);
-}
-
-template <typename TX, typename TH, int G, int NE>
+template <typename TX, typename TH, int G, int NE, int P>
 __global__ __launch_bounds__(256) void residual_norm_kernel(NormArgs a) {
-    constexpr int P = piece_elems<TX>(), NC = NE / P;
+    constexpr int NC = NE / P;
+    constexpr bool AHEAD = NE == 8;
     __shared__ float part[2][4];
     int turn = 0;
     const int lane = threadIdx.x % G;
     const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
     if (row >= a.rows) return;                       // a whole group of G lanes: G = 256 never leaves early
-    float x[NC][P];
+    const Pieces<NC> q = row_pieces<G, NC, P>(lane, a.width);
+    const int64_t start = row * a.width, gate_row = a.gate ? (row / a.rows_per_gate) * a.width : 0;
+    float x[NC][P], h[NC][P], gate[NC][P];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int col = (c * G + lane) * P;
-        load_elems<P>((const TX*)a.x + row * a.width + col, a.width - col, x[c]);
-    }
-    const int64_t gate_row = a.gate ? (row / a.rows_per_gate) * a.width : 0;
+    for (int c = 0; c < NC; ++c) load_whole<P>((const TX*)a.x + start + q.at[c], x[c]);
+    if (a.h && !a.slots)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) load_whole<P>((const TH*)a.h + start + q.at[c], h[c]);
     NormParams<NC, P> post, pre;
-    float gate[NC][P];
     auto load_gate = [&](int c) {
-        const int col = (c * G + lane) * P;
-        if (a.gate_f32) load_elems<P>((const float*)a.gate + gate_row + col, a.width - col, gate[c]);
-        else load_elems<P>((const TH*)a.gate + gate_row + col, a.width - col, gate[c]);
+        if (a.gate_f32) load_whole<P>((const float*)a.gate + gate_row + q.at[c], gate[c]);
+        else load_whole<P>((const TH*)a.gate + gate_row + q.at[c], gate[c]);
     };
-    constexpr bool AHEAD = NE == 8;
     if (AHEAD) {
-        if (a.post_weight) load_params<G, NC, P>(post, a.post_weight, a.post_bias, a, lane);
-        if (a.pre_weight) load_params<G, NC, P>(pre, a.pre_weight, a.pre_bias, a, lane);
+        if (a.post_weight) load_params(post, a.post_weight, a.post_bias, q);
+        if (a.pre_weight) load_params(pre, a.pre_weight, a.pre_bias, q);
         if (a.gate)
 #pragma unroll
             for (int c = 0; c < NC; ++c) load_gate(c);
     }
     if (a.h) {
-        float h[NC][P];
         if (a.slots) {
 #pragma unroll
             for (int c = 0; c < NC; ++c)
@@ -163,49 +176,39 @@ __global__ __launch_bounds__(256) void residual_norm_kernel(NormArgs a) {
             for (int j = 0; j < a.k; j += 2) {
                 const ChoicePair p = choice_pair(a.slots + row * a.k, a.weights + row * a.k, a.k, j, a.h_rows);
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
-                    if (p.slot[q] >= 0)
+                for (int s = 0; s < 2; ++s)
+                    if (p.slot[s] >= 0)
 #pragma unroll
                         for (int c = 0; c < NC; ++c) {
-                            const int col = (c * G + lane) * P;
                             float y[P];
-                            load_elems<P>((const TH*)a.h + (int64_t)p.slot[q] * a.width + col, a.width - col, y);
+                            load_whole<P>((const TH*)a.h + (int64_t)p.slot[s] * a.width + q.at[c], y);
 #pragma unroll
-                            for (int i = 0; i < P; ++i) h[c][i] += p.weight[q] * y[i];
+                            for (int i = 0; i < P; ++i) h[c][i] += p.weight[s] * y[i];
                         }
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int col = (c * G + lane) * P;
-                load_elems<P>((const TH*)a.h + row * a.width + col, a.width - col, h[c]);
             }
         }
         if (a.post_weight) {
-            if (!AHEAD) load_params<G, NC, P>(post, a.post_weight, a.post_bias, a, lane);
-            normalise<G, NC, P>(h, post, a, lane, part, turn);
+            if (!AHEAD) load_params(post, a.post_weight, a.post_bias, q);
+            normalise<G, NC, P>(h, post, q, a, part, turn);
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = (c * G + lane) * P;
             if (a.gate) {
                 if (!AHEAD) load_gate(c);
 #pragma unroll
                 for (int i = 0; i < P; ++i) h[c][i] *= gate_value(gate[c][i], a.gate_act);
             }
 #pragma unroll
-            for (int i = 0; i < P; ++i) x[c][i] += a.scale * h[c][i];            // zeros behind the row, like its weights
-            store_elems<P>((TX*)a.x_out + row * a.width + col, a.width - col, x[c]);
+            for (int i = 0; i < P; ++i) x[c][i] += a.scale * h[c][i];
+            if (q.own[c] < P) store_whole<P>((TX*)a.x_out + start + q.at[c], x[c]);
         }
     }
     if (a.pre_weight) {
-        if (!AHEAD) load_params<G, NC, P>(pre, a.pre_weight, a.pre_bias, a, lane);
-        normalise<G, NC, P>(x, pre, a, lane, part, turn);
+        if (!AHEAD) load_params(pre, a.pre_weight, a.pre_bias, q);
+        normalise<G, NC, P>(x, pre, q, a, part, turn);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int col = (c * G + lane) * P;
-            store_elems<P>((TH*)a.u + row * a.width + col, a.width - col, x[c]);
-        }
+        for (int c = 0; c < NC; ++c)
+            if (q.own[c] < P) store_whole<P>((TH*)a.u + start + q.at[c], x[c]);
     }
 }
 
@@ -214,45 +217,51 @@ static int launch_residual_norm(const NormArgs& a, hipStream_t stream) {
     // Lanes per row: 8 elements a lane up to 512 and in a workgroup's reach of 2048 (6000 rows of 2048 in bfloat16 with two
     // choices: 32.1 us; a wave a row 42.9 us), but a wave for up to 1024 (8160 rows, float32 x: 26.2 us, a workgroup 37.7 us)
     // unless there are too few rows to give every CU eight waves.
+    constexpr int P = 16 / (int)sizeof(TX);
     const bool few = a.rows < 2048;
-#define FD_NORM(G, NE)                                                                                                \
-    do {                                                                                                              \
-        const int64_t blocks = (a.rows + 256 / G - 1) / (256 / G);                                                    \
-        hipLaunchKernelGGL((residual_norm_kernel<TX, TH, G, NE>), dim3((unsigned)blocks), dim3(256), 0, stream, a);   \
+#define FD_NORM(G, NE, PIECE)                                                                                               \
+    do {                                                                                                                    \
+        const int64_t blocks = (a.rows + 256 / G - 1) / (256 / G);                                                          \
+        hipLaunchKernelGGL((residual_norm_kernel<TX, TH, G, NE, PIECE>), dim3((unsigned)blocks), dim3(256), 0, stream, a);  \
     } while (0)
-    if (a.width <= 128) FD_NORM(16, 8);
-    else if (a.width <= 512) FD_NORM(64, 8);
-    else if (a.width <= 1024 && !few) FD_NORM(64, 16);
-    else if (a.width <= 2048) FD_NORM(256, 8);
-    else if (a.width <= 4096) FD_NORM(256, 16);
-    else if (a.width <= 8192) FD_NORM(256, 32);
-    else FD_NORM(256, 64);
+    if (a.width < P) FD_NORM(16, 8, 1);
+    else if (a.width <= 128) FD_NORM(16, 8, P);
+    else if (a.width <= 512) FD_NORM(64, 8, P);
+    else if (a.width <= 1024 && !few) FD_NORM(64, 16, P);
+    else if (a.width <= 2048) FD_NORM(256, 8, P);
+    else if (a.width <= 4096) FD_NORM(256, 16, P);
+    else if (a.width <= 8192) FD_NORM(256, 32, P);
+    else FD_NORM(256, 64, P);
 #undef FD_NORM
     FD_LAUNCH_CHECK();
     return FD_OK;
 }
 
-// out[t] = sum_j weights[t,j] * y[slots[t,j]], terms in the order of j.  A thread owns 8 columns of a row.
-template <typename T>
+// out[t] = sum_j weights[t,j] * y[slots[t,j]], terms in the order of j.  A thread owns P columns of a row; the last piece of a
+// row is moved back to lie in it, and writes the columns that it shares a second time.
+template <typename T, int P>
 __global__ __launch_bounds__(256) void expert_combine_kernel(const T* y, int64_t y_rows, int width, const int32_t* slots, const float* weights,
                                                              int64_t rows, int k, T* out) {
     const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (row >= rows) return;
-    for (int col = (blockIdx.y * blockDim.x + threadIdx.x) * 8; col < width; col += gridDim.y * blockDim.x * 8) {
-        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int col = (blockIdx.y * blockDim.x + threadIdx.x) * P; col < width; col += gridDim.y * blockDim.x * P) {
+        const int at = min(col, width - P);
+        float acc[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) acc[i] = 0.f;
         for (int j = 0; j < k; j += 2) {
             const ChoicePair p = choice_pair(slots + row * k, weights + row * k, k, j, y_rows);
-            float v[2][8];
+            float v[2][P];
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
-                if (p.slot[q] >= 0) load8(y + (int64_t)p.slot[q] * width + col, width - col, v[q]);
+            for (int s = 0; s < 2; ++s)
+                if (p.slot[s] >= 0) load_whole<P>(y + (int64_t)p.slot[s] * width + at, v[s]);
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
-                if (p.slot[q] >= 0)
+            for (int s = 0; s < 2; ++s)
+                if (p.slot[s] >= 0)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[i] += p.weight[q] * v[q][i];
+                    for (int i = 0; i < P; ++i) acc[i] += p.weight[s] * v[s][i];
         }
-        store8(out + row * width + col, width - col, acc);
+        store_whole<P>(out + row * width + at, acc);
     }
 }
 
@@ -307,7 +316,7 @@ int fd_expert_combine(const void* y, int dtype, int64_t y_rows, int width, const
     FD_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && y_rows >= 0 && width > 0 && k > 0, "fd_expert_combine: bad shape");
     if (rows == 0) return FD_OK;
     FD_REQUIRE(slots && weights && out && (y || y_rows == 0), "fd_expert_combine: NULL pointer");
-    const int pieces = fd::ceil_div(width, 8);
+    const int per = width < 8 ? 1 : 8, pieces = fd::ceil_div(width, per);
     int bx = 1;
     while (bx < pieces && bx < 256) bx *= 2;
     const dim3 block(bx, 256 / bx);
@@ -317,8 +326,12 @@ int fd_expert_combine(const void* y, int dtype, int64_t y_rows, int width, const
     fd::ProfScope scope(fd::as_stream(stream), "expert_combine", 2.0 * rows * width * k, n * (k + 1));
     return fd::with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL((fd::expert_combine_kernel<T>), grid, block, 0, fd::as_stream(stream), (const T*)y, y_rows, width, slots, weights, rows,
-                           k, (T*)out);
+        if (per == 1)
+            hipLaunchKernelGGL((fd::expert_combine_kernel<T, 1>), grid, block, 0, fd::as_stream(stream), (const T*)y, y_rows, width, slots, weights,
+                               rows, k, (T*)out);
+        else
+            hipLaunchKernelGGL((fd::expert_combine_kernel<T, 8>), grid, block, 0, fd::as_stream(stream), (const T*)y, y_rows, width, slots, weights,
+                               rows, k, (T*)out);
         FD_LAUNCH_CHECK();
         return FD_OK;
     });

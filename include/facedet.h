@@ -395,7 +395,7 @@ int fd_expert_combine(const void* y, int dtype, int64_t y_rows, int width, const
  * without a norm; pre_weight == NULL: u is not computed.  With slots, h is the expert sum of fd_expert_combine over
  * h [h_rows, width].  The gate has gate_rows rows, each for rows / gate_rows consecutive rows of x (1: one for all; the number
  * of frames: one per frame; rows: one per row).  x may be float32 beside a 16-bit h; u has h's type.  u is computed from
- * the unrounded x_out.  x_out may be x, u may be h unless slots are given. */
+ * the unrounded x_out.  Outputs do not overlap inputs. */
 typedef struct fd_norm_args {
     const void* x;             /* [rows, width]                                    */
     const void* h;             /* [rows, width], with slots [h_rows, width], NULL  */
