@@ -214,9 +214,10 @@ __global__ __launch_bounds__(256) void residual_norm_kernel(NormArgs a) {
 
 template <typename TX, typename TH>
 static int launch_residual_norm(const NormArgs& a, hipStream_t stream) {
-    // Lanes per row: 8 elements a lane up to 512 and in a workgroup's reach of 2048 (6000 rows of 2048 in bfloat16 with two
-    // choices: 32.1 us; a wave a row 42.9 us), but a wave for up to 1024 (8160 rows, float32 x: 26.2 us, a workgroup 37.7 us)
-    // unless there are too few rows to give every CU eight waves.
+    // Lanes per row: 16 up to 256 (100000 x 256 in bfloat16: 17.8 us, a wave a row 30.9); 8 elements a lane up to 512 and, with a block's output, in a workgroup's reach of 2048 (50000 rows of 2048 in
+    // bfloat16: 163 us, a wave a row 203; 6000 with two choices: 27 and 33 us).  A wave for up to 1024 (101351 x 947: 94 us, two
+    // waves 130) and for the norm alone up to 2048 (50000 x 1900: 92 us, a workgroup 109), unless there are too few rows to
+    // give every CU eight waves.
     constexpr int P = 16 / (int)sizeof(TX);
     const bool few = a.rows < 2048;
 #define FD_NORM(G, NE, PIECE)                                                                                               \
@@ -226,8 +227,10 @@ static int launch_residual_norm(const NormArgs& a, hipStream_t stream) {
     } while (0)
     if (a.width < P) FD_NORM(16, 8, 1);
     else if (a.width <= 128) FD_NORM(16, 8, P);
+    else if (a.width <= 256) FD_NORM(16, 16, P);
     else if (a.width <= 512) FD_NORM(64, 8, P);
     else if (a.width <= 1024 && !few) FD_NORM(64, 16, P);
+    else if (a.width <= 2048 && !few && !a.h) FD_NORM(64, 32, P);
     else if (a.width <= 2048) FD_NORM(256, 8, P);
     else if (a.width <= 4096) FD_NORM(256, 16, P);
     else if (a.width <= 8192) FD_NORM(256, 32, P);

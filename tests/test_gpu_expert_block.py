@@ -343,7 +343,7 @@ def test_expert_linear_empty_and_numpy():
 # ---------------------------------------------------------------------------------------------------------------
 # weighted sum
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T,k,N", [(1, 1, 1), (3, 2, 7), (10, 2, 2048), (77, 8, 33), (500, 3, 1001), (2, 1, 9000), (1300, 4, 64)])
+@pytest.mark.parametrize("T,k,N", [(1, 1, 1), (3, 2, 7), (10, 2, 2048), (77, 8, 33), (500, 3, 1001), (9, 3, 8), (9, 3, 9), (2, 1, 9000), (1300, 4, 64)])
 def test_expert_combine(dtype, T, k, N):
     from facedetection_amd import ops
     g = _gen(T + N)
@@ -378,7 +378,7 @@ def _norm64(v, tv, w, b, layer, eps=1e-6):
     return out, tol
 
 
-NORM_WIDTHS = [1, 7, 33, 64, 128, 129, 512, 771, 1000, 1024, 1025, 2048, 2500, 4096, 5000, 8192, 9001, 16384]
+NORM_WIDTHS = [1, 3, 4, 5, 7, 8, 9, 33, 64, 128, 129, 256, 257, 511, 512, 771, 1000, 1024, 1025, 2047, 2048, 2500, 4096, 5000, 8192, 9001, 16383, 16384]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
