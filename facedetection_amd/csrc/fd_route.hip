@@ -49,7 +49,7 @@ __device__ __forceinline__ int exclusive_scan(int v, int* words, int& all) {
     return before + sum - v;
 }
 
-template <typename T, int KM>
+template <typename T, int KM, bool WHOLE>
 __global__ __launch_bounds__(2 * ROUTE_ROWS) void expert_choose_kernel(RouteArgs a) {
     constexpr int HALF = ROUTE_COLS / 2;
     __shared__ float stage[ROUTE_STAGE];
@@ -66,22 +66,39 @@ __global__ __launch_bounds__(2 * ROUTE_ROWS) void expert_choose_kernel(RouteArgs
         best[i] = -1;
     }
     float sum = 0.f, sum_at = -INFINITY;           // of exp(v - sum_at) over what the thread has seen
-    // A thread fetches 8 experts of 2 rows, 4 threads a row; the next experts are on their way while these are walked.
-    float next[2][8];
+    // A thread fetches 8 experts of 2 rows, 4 threads a row; the next experts are on their way while these are walked.  A piece
+    // that would end behind the row is moved back to its last 8 experts, so that no load stands in a branch (WHOLE: 8 or more).
+    T next[2][8];
+    const int piece = (tid & 3) * 8;
     auto fetch = [&](int c0) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int r = (tid >> 2) + i * (ROUTE_ROWS / 2), c = c0 + (tid & 3) * 8;
-            load8((const T*)a.logits + (int64_t)(row0 + r) * a.experts + c, row0 + r < a.rows ? a.experts - c : 0, next[i]);
+            const int64_t r = min(row0 + (tid >> 2) + i * (ROUTE_ROWS / 2), a.rows - 1);
+            const T* p = (const T*)a.logits + r * a.experts;
+            if (WHOLE) {
+                __builtin_memcpy(next[i], p + min(c0 + piece, a.experts - 8), sizeof(next[i]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) next[i][j] = p[min(piece + j, a.experts - 1)];
+            }
         }
     };
     fetch(0);
     for (int c0 = 0; c0 < a.experts; c0 += ROUTE_COLS) {
+        const int back = WHOLE ? max(0, c0 + piece - (a.experts - 8)) : 0;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
+            float* to = stage + ((tid >> 2) + i * (ROUTE_ROWS / 2)) * (ROUTE_COLS + 1) + piece;
+            if (back == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) stage[((tid >> 2) + i * (ROUTE_ROWS / 2)) * (ROUTE_COLS + 1) + (tid & 3) * 8 + j] = next[i][j];
+                for (int j = 0; j < 8; ++j) to[j] = (float)next[i][j];
+            } else {
+#pragma unroll
+                for (int j = 1; j < 8; ++j)
+                    if (j >= back) to[j - back] = (float)next[i][j];
+            }
+        }
         __syncthreads();
         if (c0 + ROUTE_COLS < a.experts) fetch(c0 + ROUTE_COLS);
         const int first = c0 + half * HALF, cols = min(HALF, a.experts - first);
@@ -372,11 +389,16 @@ static void launch_choose(const RouteArgs& a, hipStream_t s) {
     }
     const dim3 grid(a.blocks), block(2 * ROUTE_ROWS);
     const size_t lds = (size_t)a.experts * ROUTE_WORDS * sizeof(unsigned long long);
-    if (a.k == 1) hipLaunchKernelGGL((expert_choose_kernel<T, 1>), grid, block, lds, s, a);
-    else if (a.k == 2) hipLaunchKernelGGL((expert_choose_kernel<T, 2>), grid, block, lds, s, a);
-    else if (a.k <= 4) hipLaunchKernelGGL((expert_choose_kernel<T, 4>), grid, block, lds, s, a);
-    else if (a.k <= 8) hipLaunchKernelGGL((expert_choose_kernel<T, 8>), grid, block, lds, s, a);
-    else hipLaunchKernelGGL((expert_choose_kernel<T, 16>), grid, block, lds, s, a);
+#define FD_CHOOSE(KM, WHOLE) hipLaunchKernelGGL((expert_choose_kernel<T, KM, WHOLE>), grid, block, lds, s, a)
+    if (a.experts < 8) {
+        if (a.k <= 2) FD_CHOOSE(2, false);
+        else FD_CHOOSE(8, false);
+    } else if (a.k == 1) FD_CHOOSE(1, true);
+    else if (a.k == 2) FD_CHOOSE(2, true);
+    else if (a.k <= 4) FD_CHOOSE(4, true);
+    else if (a.k <= 8) FD_CHOOSE(8, true);
+    else FD_CHOOSE(16, true);
+#undef FD_CHOOSE
 }
 
 }  // namespace fd
