@@ -14,6 +14,7 @@
 #include "fd_conv_split_dev.h"
 #include "fd_elem.h"
 
+#include <cmath>
 #include <type_traits>
 
 namespace fd {
@@ -968,60 +969,74 @@ static bool dma_rows(const ExpertArgs& a) {
     return row % 16 == 0 && row > 128 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0 && a.wrows * row < limit && (a.rows ? a.x_rows : 256) * row < limit;
 }
 
-// Which kernel, by sizes, type and alignment (times measured in bfloat16 unless said otherwise).
+// Which kernel, by sizes, type and alignment (times in bfloat16 unless said otherwise).
 //
-// Few rows an expert: the stream kernel, for 16 rows at a time while an expert has 6 or all have 16 together (20 slots on 8
-// experts of 2 x 1024 x 2048: 14.8 us, 64 x 64 tiles 21 us; one row, 2048 x 4096: 11 against 34 us), for 32 up to 24
-// an expert (128 slots on those experts: 17.6 against 21 us; 320 slots: 31 against 24.5 us).  Long rows have eight waves a
-// workgroup (float32, the 20 slots: 31.9 us, with four 34.8 us).
+// The stream kernel for up to 4 rows an expert (20 slots on 8 experts of 2 x 1024 x 2048: 14.9 us, 32 x 64 tiles 16.2 us, 64 x 64
+// 20.6; 512 slots on 64 experts of 2 x 512 x 1024: 34.9, 28.6, 28.3 us), in float32 up to 12 (80 slots on those 8: 39.5,
+// 45, 63 us), and wherever 32 x 64 tiles would leave half of the CUs idle, since it splits K over its waves (20 slots,
+// 2048 x 4096: 11.5 and 25.8 us).  Then with 16 rows at a time up to 32 an expert, beyond with 32 (64 slots, 2048 x 4096: 18.7 and
+// 15.5 us).  Long rows have eight waves a workgroup (float32, the 20 slots: 31.9 us, with four 34.8).
 //
-// Otherwise tiles.  A CU works through ceil(tiles / CUs) of them, and one step of 128 bytes of K costs a CU (with all CUs
-// busy) 1.75, 1.48 and 1.34 us for 256, 224 and 192 x 256, 0.57 us for 128 x 128, 0.37 us for 64 x 128 and 0.27 us for 64 x 64;
-// the large ones, alone on their CU, another 3.5 to 4 us for their ends.  Large tiles win on many rows an expert (32768 rows,
-// 2048 x 4096: 1.22 PFLOP/s for 256 x 256, 0.93, 0.73 and 0.51 for the small ones), a little smaller ones when the last round
-// of tiles is nearly empty (12000 slots on 8 experts of 2048 x 2048: 126 us with 256 rows, 113 with 224, 133 with 192; 8000 on
-// 32 experts of 2 x 1024 x 1024: 71, 64, 60 us), small ones when an expert has few (1200 slots on 16 such experts: 29 us with
-// 256 x 256, 21, 20 and 20 us).  The large ones take outputs in eights and three steps or more.
-// Through registers, for rows that are not aligned, it is 1.07 us for 128 x 128 and 0.41 us for 64 x 64 (62682 slots,
-// 1448 x 1001: 394 and 583 us; 2331 slots, 333 x 1001: 34 and 17 us), and with less than a 64 x 64 tile a CU 32 x 64 spreads
-// the loads (400 slots, 733 x 1001: 12.2 us, 14.5 with 64 x 64).  In float32 the matrix units are slow enough (1/16)
+// Otherwise tiles.  A CU works through ceil(tiles / CUs) of them, and one step of 128 bytes of K costs a CU (with all CUs busy)
+// 1.75, 1.48 and 1.34 us for 256, 224 and 192 x 256, 0.57 us for 128 x 128, 0.37 us for 64 x 128 and 0.27 us for 64 x 64, but a step
+// of a tile is not shorter than its loads take; the large ones, alone on their CU, need another 3.5 to 4 us for their ends.
+// Large tiles win on many rows an expert (32768 rows, 2048 x 4096: 1.22 PFLOP/s for 256 x 256, 0.93, 0.73 and 0.51 for the small
+// ones), a little smaller ones when the last round of tiles is nearly empty (12000 slots on 8 experts of 2048 x 2048: 126 us
+// with 256 rows, 113 with 224, 133 with 192; 8000 on 32 experts of 2 x 1024 x 1024: 71, 64, 60 us), small ones when an expert
+// has few (1200 slots on 16 such experts: 29 us with 256 x 256, 21, 20 and 20 us).  The large ones take outputs in eights
+// and three steps or more.
+// Through registers, for rows that are not aligned, it is 1.15 us for 128 x 128, 0.45 for 64 x 64 and 0.33 for 32 x 64 (62682 slots,
+// 1448 x 1001: 394 and 583 us for the first two; 2331 slots, 333 x 1001: 34, 16.0, 15.2 us; 41076 slots on 33 experts of
+// 2 x 47 x 3191: 122, 146, 184 us).  32 x 64 through registers has the shortest step of a single tile and is offered
+// for aligned rows too, 0.24 us a step (796 slots on 50 experts of 1547 x 832: 29.9 us, 64 x 64 33 to 36, 64 x 128 31.3; 320 on
+// 8 experts of 2 x 1024 x 2048: 19.3, 21.0 us).  In float32 the matrix units are slow enough (1/16)
 // that every tile reaches the same rate (126 TFLOP/s) and the smallest wastes the least.
 template <typename T>
 static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
+    typedef int (*Launch)(const ExpertArgs&, hipStream_t);
     const int64_t groups = a.experts < a.slots ? a.experts : a.slots, row_bytes = (int64_t)a.K * sizeof(T);
-    if (a.slots <= 16 || a.slots <= 6 * groups)
-        return row_bytes < 8192 ? launch_expert_stream<T, 1, 4, 4>(a, stream) : launch_expert_stream<T, 1, 8, 4>(a, stream);
-    if (a.slots <= 32 || a.slots <= 24 * groups) return launch_expert_stream<T, 2, 4, 4>(a, stream);
-    const int steps = ceil_div(row_bytes, 128);
-    auto cost = [&](int bm, int bn, double step, double ends) {
+    const int steps = ceil_div(row_bytes, 128), cus = compute_units();
+    auto tiles_of = [&](int bm, int bn) {
         // a group ends in half a tile on average, a single one where it does
         const double rows = groups == 1 ? ceil_div(a.slots, bm) : a.slots / (double)bm + groups / 2.0;
-        return ceil(rows * ceil_div(a.wrows, bn) / compute_units()) * (steps * step + ends);
+        return rows * ceil_div(a.wrows, bn);
     };
-    if (!dma_rows<T>(a)) {
-        if (cost(64, 64, 1.0, 0.0) <= steps) return launch_expert_tile<T, 32, 64, 2, 4>(a, stream);
-        if (sizeof(T) == 4 || cost(64, 64, 0.41, 0.3) <= cost(128, 128, 1.07, 1.0)) return launch_expert_tile<T, 64, 64, 2, 4>(a, stream);
-        return launch_expert_tile<T, 128, 128, 1, 2>(a, stream);
+    if (a.slots <= (sizeof(T) == 4 ? 12 : 4) * groups || (a.slots <= 64 * groups && tiles_of(32, 64) < cus / 2)) {
+        if (a.slots > 32 * groups) return launch_expert_stream<T, 2, 4, 4>(a, stream);
+        return row_bytes < 8192 ? launch_expert_stream<T, 1, 4, 4>(a, stream) : launch_expert_stream<T, 1, 8, 4>(a, stream);
     }
+    double least = 0.0;
+    Launch best = nullptr;
+    // a step costs a CU `step` for each of its tiles but takes `load` at least; `ends`: a tile's start and end
+    auto offer = [&](int bm, int bn, double step, double load, double ends, Launch launch) {
+        const double rounds = ceil(tiles_of(bm, bn) / cus), cost = steps * fmax(rounds * step, load) + rounds * ends;
+        if (!best || cost < least) {
+            least = cost;
+            best = launch;
+        }
+    };
+    const bool aligned = dma_rows<T>(a);
     if constexpr (sizeof(T) == 4) {
-        return launch_expert_dma<T, 64, 64, 2, 2, 4>(a, stream);
+        offer(32, 64, 0.30, 0.63, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 32, 64, 2, 4>(p, q); });
+        if (aligned) offer(64, 64, 0.50, 0.90, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 64, 2, 2, 4>(p, q); });
+        else offer(64, 64, 0.55, 0.90, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 64, 64, 2, 4>(p, q); });
     } else {
-        struct {
-            double cost;
-            int (*launch)(const ExpertArgs&, hipStream_t);
-        } tiles[] = {
-            {cost(256, 256, 1.75, 3.9), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 8>(p, q); }},
-            {cost(224, 256, 1.48, 3.6), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 7>(p, q); }},
-            {cost(192, 256, 1.34, 3.4), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 6>(p, q); }},
-            {cost(128, 128, 0.57, 1.0), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 128, 128, 2, 2, 2>(p, q); }},
-            {cost(64, 128, 0.37, 0.5), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 128, 2, 2, 3>(p, q); }},
-            {cost(64, 64, 0.27, 0.3), [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 64, 2, 2, 4>(p, q); }},
-        };
-        int best = a.N % 8 == 0 && row_bytes > 256 ? 0 : 3;
-        for (int i = best + 1; i < 6; ++i)
-            if (tiles[i].cost < tiles[best].cost) best = i;
-        return tiles[best].launch(a, stream);
+        offer(32, 64, aligned ? 0.24 : 0.33, 0.36, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 32, 64, 2, 4>(p, q); });
+        if (!aligned) {
+            offer(64, 64, 0.45, 0.45, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 64, 64, 2, 4>(p, q); });
+            offer(128, 128, 1.15, 1.15, 1.0, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 128, 128, 1, 2>(p, q); });
+        } else {
+            offer(64, 64, 0.27, 0.55, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 64, 2, 2, 4>(p, q); });
+            offer(64, 128, 0.37, 0.72, 0.5, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 128, 2, 2, 3>(p, q); });
+            offer(128, 128, 0.57, 0.80, 1.0, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 128, 128, 2, 2, 2>(p, q); });
+            if (a.N % 8 == 0 && row_bytes > 256) {
+                offer(192, 256, 1.34, 1.34, 3.4, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 6>(p, q); });
+                offer(224, 256, 1.48, 1.48, 3.6, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 7>(p, q); });
+                offer(256, 256, 1.75, 1.75, 3.9, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 8>(p, q); });
+            }
+        }
     }
+    return best(a, stream);
 }
 
 }  // namespace fd
