@@ -14,6 +14,7 @@
 #include "fd_conv_split_dev.h"
 #include "fd_elem.h"
 
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -111,7 +112,7 @@ __device__ __forceinline__ float gelu(float v) {
 
 template <typename T>
 __device__ __forceinline__ float activate(float v, int act) {
-    if (act == FD_ACT_RELU) return fmaxf(v, 0.f);
+    if (act == FD_ACT_RELU) return v < 0.f ? 0.f : v;         // not a number stays so
     // hardware exp2 and reciprocal, one unit each: exp(-v) is off by |v| * 2^-24 of itself, v * sigmoid(v) by less than
     // 2^-24 * (|v| + 1) for every v, below the bound of the sum in front of it
     if (act == FD_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * v));
@@ -440,9 +441,10 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void expert_dma_kernel(ExpertArg
     // what is loaded: a tile's rows and weights, their buffers, and whether the lane's piece of the step lies behind K
     __amdgpu_buffer_rsrc_t xr, wr;
     auto aim = [&](const Tile& t) {
-        // without a row list the rows of a tile are a range of their own, so x may be of any size
+        // without a row list the rows of a tile are a range of their own, so x may be of any size; a row at least, so that the
+        // offset of a step never passes the end, which the range check subtracts it from
         xr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.x + (a.rows ? 0 : (int64_t)t.m0 * row_bytes)), 0,
-                                               a.rows ? x_bytes : (unsigned)(t.m1 - t.m0) * row_bytes, 0x00020000);
+                                               a.rows ? x_bytes : (unsigned)max(t.m1 - t.m0, 1) * row_bytes, 0x00020000);
         wr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.w + (int64_t)t.e * a.wrows * row_bytes), 0, (unsigned)a.wrows * row_bytes,
                                                0x00020000);
     };
@@ -676,9 +678,10 @@ __global__ __launch_bounds__(512, 2) void expert_wide_kernel(ExpertArgs a, unsig
     // what is loaded: a tile's rows and weights, their buffers, and whether the lane's piece of the step lies behind K
     __amdgpu_buffer_rsrc_t xr, wr;
     auto aim = [&](const Tile& t) {
-        // without a row list the rows of a tile are a range of their own, so x may be of any size
+        // without a row list the rows of a tile are a range of their own, so x may be of any size; a row at least, so that the
+        // offset of a step never passes the end, which the range check subtracts it from
         xr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.x + (a.rows ? 0 : (int64_t)t.m0 * row_bytes)), 0,
-                                               a.rows ? x_bytes : (unsigned)(t.m1 - t.m0) * row_bytes, 0x00020000);
+                                               a.rows ? x_bytes : (unsigned)max(t.m1 - t.m0, 1) * row_bytes, 0x00020000);
         wr = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.w + (int64_t)t.e * a.wrows * row_bytes), 0, (unsigned)a.wrows * row_bytes,
                                                0x00020000);
     };
@@ -886,11 +889,13 @@ static double expert_bytes(const ExpertArgs& a) {
 
 // CUs of the current device, asked for once.
 static int compute_units() {
-    static int cus[64];
-    int dev = 0;
+    static std::atomic<int> known[64];
+    int dev = 0, cus = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-    if (!cus[dev] && hipDeviceGetAttribute(&cus[dev], hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 256;
-    return cus[dev];
+    if ((cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
+    known[dev].store(cus, std::memory_order_relaxed);
+    return cus;
 }
 
 // Workgroups for tiles of BM slots: as many as run at once, a multiple of the 8 XCDs; 0 with an error if the tiles cannot
@@ -966,7 +971,7 @@ static int launch_expert_stream(ExpertArgs a, hipStream_t stream) {
 template <typename T>
 static bool dma_rows(const ExpertArgs& a) {
     const int64_t row = (int64_t)a.K * sizeof(T), limit = int64_t(1) << 31;
-    return row % 16 == 0 && row > 128 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0 && a.wrows * row < limit && (a.rows ? a.x_rows : 256) * row < limit;
+    return a.x_rows > 0 && row % 16 == 0 && row > 128 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0 && a.wrows * row < limit && (a.rows ? a.x_rows : 256) * row < limit;
 }
 
 // Which kernel, by sizes, type and alignment (times in bfloat16 unless said otherwise).

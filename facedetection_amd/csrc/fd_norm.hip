@@ -117,6 +117,14 @@ __device__ __forceinline__ void normalise(float (&v)[NC][P], const NormParams<NC
         for (int i = 0; i < P; ++i) v[c][i] = v[c][i] * r * p.weight[c][i] + p.bias[c][i];
 }
 
+// The index of a workgroup, and the grid for `blocks` of them: a grid dimension holds fewer than 2^32 threads.
+constexpr int64_t GRID_BLOCKS = 1 << 23;
+inline dim3 block_grid(int64_t blocks, int columns = 1) {
+    const int64_t x = blocks < GRID_BLOCKS ? blocks : GRID_BLOCKS;
+    return dim3((unsigned)x, columns, (unsigned)((blocks + x - 1) / x));
+}
+__device__ __forceinline__ int64_t block_index() { return (int64_t)blockIdx.z * gridDim.x + blockIdx.x; }
+
 // Two of a row's choices, so that both are asked for before either is waited for; -1 for a choice that is not made.
 struct ChoicePair {
     int32_t slot[2];
@@ -145,7 +153,7 @@ __global__ __launch_bounds__(256) void residual_norm_kernel(NormArgs a) {
     __shared__ float part[2][4];
     int turn = 0;
     const int lane = threadIdx.x % G;
-    const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int64_t row = block_index() * (256 / G) + threadIdx.x / G;
     if (row >= a.rows) return;                       // a whole group of G lanes: G = 256 never leaves early
     const Pieces<NC> q = row_pieces<G, NC, P>(lane, a.width);
     const int64_t start = row * a.width, gate_row = a.gate ? (row / a.rows_per_gate) * a.width : 0;
@@ -214,16 +222,16 @@ __global__ __launch_bounds__(256) void residual_norm_kernel(NormArgs a) {
 
 template <typename TX, typename TH>
 static int launch_residual_norm(const NormArgs& a, hipStream_t stream) {
-    // Lanes per row: 16 up to 256 (100000 x 256 in bfloat16: 17.8 us, a wave a row 30.9); 8 elements a lane up to 512 and, with a block's output, in a workgroup's reach of 2048 (50000 rows of 2048 in
-    // bfloat16: 163 us, a wave a row 203; 6000 with two choices: 27 and 33 us).  A wave for up to 1024 (101351 x 947: 94 us, two
-    // waves 130) and for the norm alone up to 2048 (50000 x 1900: 92 us, a workgroup 109), unless there are too few rows to
-    // give every CU eight waves.
+    // Lanes per row: 16 up to 256 (100000 x 256 in bfloat16: 17.8 us, a wave a row 30.9); 8 elements a lane up to 512 and,
+    // with a block's output, in a workgroup's reach of 2048 (50000 rows of 2048 in bfloat16: 163 us, a wave a row 203; 6000
+    // with two choices: 27 and 33 us).  A wave for up to 1024 (101351 x 947: 94 us, two waves 130) and for the norm alone up
+    // to 2048 (50000 x 1900: 92 us, a workgroup 109), unless there are too few rows to give every CU eight waves.
     constexpr int P = 16 / (int)sizeof(TX);
     const bool few = a.rows < 2048;
 #define FD_NORM(G, NE, PIECE)                                                                                               \
     do {                                                                                                                    \
         const int64_t blocks = (a.rows + 256 / G - 1) / (256 / G);                                                          \
-        hipLaunchKernelGGL((residual_norm_kernel<TX, TH, G, NE, PIECE>), dim3((unsigned)blocks), dim3(256), 0, stream, a);  \
+        hipLaunchKernelGGL((residual_norm_kernel<TX, TH, G, NE, PIECE>), block_grid(blocks), dim3(256), 0, stream, a);      \
     } while (0)
     if (a.width < P) FD_NORM(16, 8, 1);
     else if (a.width <= 128) FD_NORM(16, 8, P);
@@ -245,7 +253,7 @@ static int launch_residual_norm(const NormArgs& a, hipStream_t stream) {
 template <typename T, int P>
 __global__ __launch_bounds__(256) void expert_combine_kernel(const T* y, int64_t y_rows, int width, const int32_t* slots, const float* weights,
                                                              int64_t rows, int k, T* out) {
-    const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    const int64_t row = block_index() * blockDim.y + threadIdx.y;
     if (row >= rows) return;
     for (int col = (blockIdx.y * blockDim.x + threadIdx.x) * P; col < width; col += gridDim.y * blockDim.x * P) {
         const int at = min(col, width - P);
@@ -324,7 +332,7 @@ int fd_expert_combine(const void* y, int dtype, int64_t y_rows, int width, const
     while (bx < pieces && bx < 256) bx *= 2;
     const dim3 block(bx, 256 / bx);
     const int gy = fd::ceil_div(pieces, bx);
-    const dim3 grid((unsigned)((rows + block.y - 1) / block.y), gy < 65535 ? gy : 65535);
+    const dim3 grid = fd::block_grid((rows + block.y - 1) / block.y, gy < 65535 ? gy : 65535);
     const double n = (double)rows * width * fd::dtype_bytes(dtype);
     fd::ProfScope scope(fd::as_stream(stream), "expert_combine", 2.0 * rows * width * k, n * (k + 1));
     return fd::with_dtype(dtype, [&](auto t) {

@@ -10,7 +10,8 @@
 // best in registers, which takes 32 rows a wave where a wave-wide arg-max would take 6 cross-lane steps a choice for one
 // row; the first thread then takes the other's in.  A row's experts are distinct, so
 // the rank of a choice among its workgroup's choices of that expert is a population count over one bit per row:
-// set with LDS atomics, whose order does not show.  Workgroups are joined by a second launch that sums their counts.
+// set with LDS atomics, whose order does not show.  Workgroups are joined by a second launch that sums their counts; where
+// there are many, whose sums would grow with the square of the rows, by a third between the two that scans them.
 #include "fd_elem.h"
 
 namespace fd {
@@ -18,6 +19,7 @@ namespace fd {
 constexpr int ROUTE_ROWS = 512;            // rows of a workgroup; two threads a row choose, one places
 constexpr int ROUTE_COLS = 32;             // experts staged at a time
 constexpr int ROUTE_WORDS = ROUTE_ROWS / 64;
+constexpr int ROUTE_SCAN = 512;            // workgroups from which on their counts are scanned
 constexpr int ROUTE_STAGE = ROUTE_ROWS * (ROUTE_COLS + 2);   // rows of 33 words; later 2 words a choice and 2 more of a row
 
 struct RouteArgs {
@@ -25,7 +27,7 @@ struct RouteArgs {
     const uint8_t* mask;
     int rows, experts, k, normalize, blocks;
     float* weights;
-    int32_t *chosen, *slots, *offsets, *source, *counts;     // counts [blocks, experts]: the workspace
+    int32_t *chosen, *slots, *offsets, *source, *counts;     // counts [blocks, experts], scanned [blocks + 1, experts]: the workspace
 };
 
 // Exclusive scan of `v` over the workgroup's first 512 threads, in `words` (an int of LDS a wave).  `all`: the sum.
@@ -320,14 +322,43 @@ __global__ __launch_bounds__(2 * ROUTE_ROWS) void expert_choose_few_kernel(Route
     }
 }
 
-// Adds to every choice's rank the choices of earlier experts and of earlier workgroups.
+// The counts of each expert become those of all earlier workgroups, with the sum behind the last.  A workgroup takes 16 experts
+// (64-byte pieces of the rows), 64 threads share one.
+__global__ __launch_bounds__(1024) void expert_scan_kernel(RouteArgs a) {
+    constexpr int PARTS = 64, U = 16;
+    __shared__ int sums[PARTS][17];
+    const int lane = threadIdx.x & 15, part = threadIdx.x >> 4, e = min((int)blockIdx.x * 16 + lane, a.experts - 1);
+    const bool mine = blockIdx.x * 16 + lane < a.experts;
+    const int each = (a.blocks + PARTS - 1) / PARTS, b0 = min(part * each, a.blocks), b1 = min(b0 + each, a.blocks);
+    int32_t* counts = a.counts + e;
+    int n = 0;
+#pragma unroll 16
+    for (int b = b0; b < b1; ++b) n += counts[(int64_t)b * a.experts];
+    sums[part][lane] = n;
+    __syncthreads();
+    int at = 0;
+    for (int p = 0; p < part; ++p) at += sums[p][lane];
+    if (!mine) return;
+    for (int b = b0; b < b1; b += U) {
+        int c[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) c[u] = counts[(int64_t)min(b + u, b1 - 1) * a.experts];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (b + u < b1) {
+                counts[(int64_t)(b + u) * a.experts] = at;
+                at += c[u];
+            }
+    }
+    if (part == PARTS - 1) counts[(int64_t)a.blocks * a.experts] = at;
+}
+
+// Adds to every choice's rank the choices of earlier experts and of earlier workgroups.  Up to ROUTE_SCAN workgroups each sums
+// the counts of all (SUMS).
+template <bool SUMS>
 __global__ __launch_bounds__(ROUTE_ROWS) void expert_place_kernel(RouteArgs a) {
-    __shared__ int before[ROUTE_ROWS], total[ROUTE_ROWS], words[ROUTE_WORDS];
+    __shared__ int before[ROUTE_ROWS], words[ROUTE_WORDS];
     const int t = threadIdx.x;
-    // 512 / lanes threads share an expert, each sums every (512 / lanes)-th workgroup
-    int lanes = 1;
-    while (lanes < a.experts) lanes *= 2;
-    const int e = t & (lanes - 1), part = t / lanes, parts = ROUTE_ROWS / lanes;
     // the row's first choices are asked for before the counts, whose sums they wait for
     const int row = blockIdx.x * ROUTE_ROWS + t;
     int c4[4], r4[4];
@@ -338,24 +369,34 @@ __global__ __launch_bounds__(ROUTE_ROWS) void expert_place_kernel(RouteArgs a) {
         r4[j] = is ? a.slots[(int64_t)row * a.k + j] : -1;
     }
     int b0 = 0, all = 0;
-    if (e < a.experts) {
+    if (SUMS) {
+        // 512 / lanes threads share an expert, each sums every (512 / lanes)-th workgroup
+        __shared__ int total[ROUTE_ROWS];
+        int lanes = 1;
+        while (lanes < a.experts) lanes *= 2;
+        const int e = t & (lanes - 1), part = t / lanes, parts = ROUTE_ROWS / lanes;
+        if (e < a.experts) {
 #pragma unroll 16
-        for (int b = part; b < a.blocks; b += parts) {
-            const int n = a.counts[(int64_t)b * a.experts + e];
-            all += n;
-            if (b < (int)blockIdx.x) b0 += n;
+            for (int b = part; b < a.blocks; b += parts) {
+                const int n = a.counts[(int64_t)b * a.experts + e];
+                all += n;
+                if (b < (int)blockIdx.x) b0 += n;
+            }
         }
+        before[t] = b0;
+        total[t] = all;
+        __syncthreads();
+        b0 = all = 0;
+        if (t < a.experts)
+            for (int p = 0; p < parts; ++p) {
+                b0 += before[p * lanes + t];
+                all += total[p * lanes + t];
+            }
+        __syncthreads();
+    } else if (t < a.experts) {
+        b0 = a.counts[(int64_t)blockIdx.x * a.experts + t];
+        all = a.counts[(int64_t)a.blocks * a.experts + t];
     }
-    before[t] = b0;
-    total[t] = all;
-    __syncthreads();
-    b0 = all = 0;
-    if (t < a.experts)
-        for (int p = 0; p < parts; ++p) {
-            b0 += before[p * lanes + t];
-            all += total[p * lanes + t];
-        }
-    __syncthreads();
     int routed;
     const int first = exclusive_scan(all, words, routed);
     before[t] = first + b0;
@@ -407,7 +448,7 @@ extern "C" {
 
 int64_t fd_expert_route_workspace(int64_t rows, int experts) {
     const int64_t blocks = (rows + fd::ROUTE_ROWS - 1) / fd::ROUTE_ROWS;
-    return blocks > 1 ? blocks * experts * (int64_t)sizeof(int32_t) : 0;
+    return blocks > 1 ? (blocks + (blocks > fd::ROUTE_SCAN)) * experts * (int64_t)sizeof(int32_t) : 0;
 }
 
 int fd_expert_route(const void* logits, int dtype, int64_t rows, int experts, int k, const uint8_t* mask, int normalize, float* weights,
@@ -433,7 +474,14 @@ int fd_expert_route(const void* logits, int dtype, int64_t rows, int experts, in
         fd::launch_choose<decltype(t)>(a, fd::as_stream(stream));
         FD_LAUNCH_CHECK();
         if (a.blocks > 1) {
-            hipLaunchKernelGGL(fd::expert_place_kernel, dim3(a.blocks), dim3(fd::ROUTE_ROWS), 0, fd::as_stream(stream), a);
+            const dim3 grid(a.blocks), block(fd::ROUTE_ROWS);
+            if (a.blocks <= fd::ROUTE_SCAN) {
+                hipLaunchKernelGGL(fd::expert_place_kernel<true>, grid, block, 0, fd::as_stream(stream), a);
+            } else {
+                hipLaunchKernelGGL(fd::expert_scan_kernel, dim3(fd::ceil_div(experts, 16)), dim3(1024), 0, fd::as_stream(stream), a);
+                FD_LAUNCH_CHECK();
+                hipLaunchKernelGGL(fd::expert_place_kernel<false>, grid, block, 0, fd::as_stream(stream), a);
+            }
             FD_LAUNCH_CHECK();
         }
         return FD_OK;

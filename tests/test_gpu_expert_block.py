@@ -606,3 +606,139 @@ def test_same_bits_every_time():
         if first is not None:
             assert all(torch.equal(a, b) for a, b in zip(out, first))
         first = out
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# more than 2^31 bytes, elements or threads, and values that are no numbers
+def test_block_norm_of_more_rows_than_a_grid_dimension_has_threads():
+    from facedetection_amd import ops
+    T = 2 ** 28 + 5                                            # 16 lanes a row: 2^32 threads and some
+    x = torch.ones((T, 1), dtype=torch.float16, device="cuda")
+    x[-3:, 0] = torch.tensor([0.0, -3.0, 0.5], device="cuda")
+    x[2 ** 27 - 1:2 ** 27 + 2, 0] = -2.0
+    u = ops.block_norm(x, torch.full((1,), 2.0, device="cuda"), bias=torch.full((1,), 1.0, device="cuda"))
+    # x / sqrt(x^2 + 1e-6) is 1 to 2e-6 (at 0.5): 3, -1 and 1, to half a step of float16 behind it
+    want = 1.0 + 2.0 * torch.sign(x)
+    assert float((u - want).abs().max()) <= 2.0 ** -9
+
+
+def test_expert_combine_of_more_rows_than_a_grid_dimension_has_threads():
+    from facedetection_amd import ops
+    if torch.cuda.mem_get_info()[0] < 100 * 2 ** 30:
+        pytest.skip("an output of 64 GiB")
+    T, N = 2 ** 24 + 3, 2048                                   # a workgroup of 256 a row
+    y = torch.randn((4, N), generator=_gen(1), device="cuda").half()
+    slots = (torch.arange(T, dtype=torch.int32, device="cuda") % 5 - 1)[:, None].contiguous()
+    out = ops.expert_combine(y, slots, torch.full((T, 1), 0.5, device="cuda"))
+    for at in (0, 2 ** 23 - 2, T - 6):
+        want = torch.where(slots[at:at + 6] >= 0, 0.5 * y[slots[at:at + 6, 0].long().clamp(min=0)].float(), 0.0).half()
+        assert torch.equal(out[at:at + 6], want)
+    del out
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("T,E,k,masked", [(262144, 9, 2, True), (262145, 9, 2, False), (300001, 100, 4, True), (270000, 512, 3, False), (1300000, 2, 1, True),
+                                          (700003, 17, 9, False)])
+def test_route_of_many_rows(T, E, k, masked):
+    """Several hundred workgroups and more, whose counts are joined another way, against stable sorts."""
+    from facedetection_amd import ops
+    g = _gen(T + E)
+    logits = torch.randn((T, E), generator=g, device="cuda")
+    mask = torch.rand((T,), generator=g, device="cuda") < 0.6 if masked else None
+    r = ops.expert_route(logits, k, mask=mask)
+    by, chosen = logits.sort(dim=1, descending=True, stable=True)
+    weights, chosen = torch.softmax(by[:, :k].double(), 1), chosen[:, :k].int()
+    if masked:
+        weights, chosen = weights * mask[:, None], torch.where(mask[:, None], chosen, -1)
+    assert torch.equal(r.experts, chosen)
+    assert float((r.weights - weights).abs().max()) <= (k + 16 + 2.0 ** 7) * U
+    flat = torch.where(chosen < 0, E, chosen).reshape(-1)
+    by, order = flat.sort(stable=True)
+    assert torch.equal(r.offsets, torch.searchsorted(by, torch.arange(E + 1, dtype=torch.int32, device="cuda")).int())
+    n = int(r.offsets[-1])
+    assert torch.equal(r.rows[:n], (order[:n] // k).int()) and bool((r.rows[n:] == -1).all())
+    slots = torch.full_like(flat, -1)
+    slots[order[:n]] = torch.arange(n, dtype=torch.int32, device="cuda")
+    assert torch.equal(r.slots.reshape(-1), slots)
+
+
+@pytest.mark.parametrize("dtype,bits,quiet", [(torch.float32, torch.int32, 0x7f800001), (torch.float16, torch.int16, 0x7c01),
+                                              (torch.bfloat16, torch.int16, 0x7f81)])
+@pytest.mark.parametrize("T", [40, 700])
+def test_route_signalling_nan_is_not_chosen(dtype, bits, quiet, T):
+    logits = torch.randn((T, 12), generator=_gen(T), device="cuda").to(dtype)
+    logits.view(bits)[::3, 4] = quiet
+    logits.view(bits)[1::7, :11] = quiet
+    assert int(torch.isnan(logits).sum()) > T // 3
+    for normalize in (True, False):
+        _check_route(logits, 3, None, normalize)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,K,N", [(3, 40, 24), (500, 40, 72), (3000, 256, 256), (3000, 251, 129), (66000, 192, 2048)])
+def test_expert_linear_nan_passes_every_activation(dtype, T, K, N):
+    from facedetection_amd import ops
+    g = _gen(T)
+    x, w = torch.randn((T, K), generator=g, device="cuda").to(dtype), torch.randn((1, 2 * N, K), generator=g, device="cuda").to(dtype)
+    off = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    x[T // 2, K // 3] = math.nan
+    for act in (None, "relu", "silu", "gelu"):
+        for gated in (False, True):
+            y = ops.expert_linear(x, w, off, activation=act, gated=gated)
+            bad = torch.isnan(y)
+            assert bool(bad[T // 2].all()) and int(bad.sum()) == y.shape[1]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("S,N", [(3, 40), (700, 200), (50000, 1024)])
+def test_expert_linear_of_no_rows_at_all(dtype, S, N):
+    """x has no rows: every index lies outside of it, and a slot of an expert is the activation of its bias."""
+    from facedetection_amd import ops
+    g = _gen(S)
+    w, b = torch.randn((2, N, 512), generator=g, device="cuda").to(dtype), torch.randn((2, N), generator=g, device="cuda").to(dtype)
+    off = torch.tensor([0, S // 3, S - 1], dtype=torch.int32, device="cuda")
+    rows = torch.arange(S, dtype=torch.int32, device="cuda") - 1
+    y = ops.expert_linear(torch.empty((0, 512), dtype=dtype, device="cuda"), w, off, rows=rows, bias=b, activation="relu")
+    want = torch.cat([b[0].relu().expand(S // 3, N), b[1].relu().expand(S - 1 - S // 3, N), torch.zeros((1, N), dtype=dtype, device="cuda")])
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("K,N,S,gather,per", [
+    (1024, 64, 2 ** 22 + 77, False, 1), (1024, 64, 3000, True, 1), (1021, 64, 3000, True, 1), (1024, 1024, 40000, True, 1),
+    (64, 1024, 2 ** 21 + 300, False, 1), (8, 1000, 2 ** 22 + 9, False, 1), (1024, 24, 5, True, 1), (512, 512, 2 ** 22 + 500, False, 2)])
+def test_expert_linear_beyond_31_bits(K, N, S, gather, per):
+    """x or y of more than 2^31 bytes or elements: slots at both ends and in the middle, rows at the end of x."""
+    from facedetection_amd import ops
+    g = _gen(K + N)
+    T = 2 ** 22 + 1234 if gather else S
+    x = torch.empty((T, K), dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    w = (torch.randn((per, N, K), generator=g, device="cuda") / math.sqrt(K)).bfloat16()
+    bias = torch.randn((per, N), generator=g, device="cuda").bfloat16()
+    rows = None
+    if gather:
+        rows = (T - 1 - torch.randint(0, T, (S,), generator=g, device="cuda") // 3).int()
+        rows[0], rows[S // 2], rows[-2] = 0, T - 1, T
+    bound = torch.tensor([0] + [(S - 1) * (e + 1) // per for e in range(per)], dtype=torch.int32, device="cuda")
+    y = ops.expert_linear(x, w, bound, rows=rows, bias=bias)
+    assert y.shape == (S, N) and bool((y[-1] == 0).all())
+    pick = torch.cat([torch.arange(0, min(S, 300)), torch.arange(S // 2 - min(S // 2, 150), S // 2 + min(S // 2, 150)),
+                      torch.arange(max(0, S - 300), S - 1)]).unique().cuda()
+    src = pick if rows is None else rows[pick].long()
+    xs = torch.where((src < T)[:, None], x[src.clamp(max=T - 1)], 0.0)
+    at = torch.searchsorted(pick, bound[1:].long()).int()
+    _close(y[pick], *_linear64(xs, w, torch.cat([torch.zeros_like(at[:1]), at]), None, bias, None, False))
+
+
+# more kinds of tiles: one row list entry more or less than a tile, more than 64 experts, two and three steps of K, and the
+# widths at which another tile is the cheaper one
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", [
+    (8000, 2, 70, 512, 264, "silu", True, True, True, 0.3, 0.1), (20000, 2, 130, 192, 520, None, False, True, True, 0.3, 0.02),
+    (3000, 2, 16, 128, 512, "silu", True, False, True, 0.3, 0.0), (12000, 1, 8, 512, 2048, None, False, True, True, 0.1, 0.0),
+    (4000, 2, 32, 1024, 1024, "silu", True, False, True, 0.5, 0.0), (600, 2, 16, 512, 512, "gelu", False, False, False, 0.5, 0.1),
+    (398, 2, 50, 416, 1003, "relu", False, True, True, 0.5, 0.0), (64, 1, 1, 2048, 256, None, False, True, True, 0.0, 0.0),
+    (20, 2, 2, 4104, 100, "silu", True, True, True, 0.0, 0.0), (3000, 1, 4, 1001, 300, None, False, False, True, 0.5, 0.0),
+    (30000, 2, 2, 249, 448, "gelu", False, True, True, 0.5, 0.0), (257, 1, 1, 192, 520, None, True, False, True, 0.0, 0.0),
+], ids=lambda c: "x".join(str(v) for v in c[:5]))
+def test_expert_linear_other_tiles(dtype, case):
+    test_expert_linear(dtype, case)
