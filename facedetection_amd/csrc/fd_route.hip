@@ -5,11 +5,11 @@
 //   weights[t,j] = exp(l_j - l_0) / sum, the sum over the row's choices (normalize) or over all its experts
 //   slots[t,j]   = position of the choice among all choices sorted by (expert, t);  rows[slots[t,j]] = t
 //
-// Bound by the read of the logits, with the walk close behind it.  Two threads share a row: each walks its half of every 32
-// experts through LDS (staged by coalesced loads, 33 words a row so that the walk has no bank conflicts) and keeps its k
-// best in registers, which takes 32 rows a wave where a wave-wide arg-max would take 6 cross-lane steps a choice for one
-// row; the first thread then takes the other's in.  A row's experts are distinct, so
-// the rank of a choice among its workgroup's choices of that expert is a population count over one bit per row:
+// Bound by the read of the logits, with the walk close behind it (130560 rows of 64 float32 logits, 4 choices of a softmax
+// over all, with mask: 19 us for 33 MB).  Two threads share a row: each walks its half of every 32 experts through LDS
+// (staged by coalesced loads, 33 words a row so that the walk has no bank conflicts) and keeps its k best in registers; the
+// first thread then takes the other's in.  Where the rows are too few for that, a wave takes one.  A row's experts are
+// distinct, so the rank of a choice among its workgroup's choices of that expert is a population count over one bit per row:
 // set with LDS atomics, whose order does not show.  Workgroups are joined by a second launch that sums their counts; where
 // there are many, whose sums would grow with the square of the rows, by a third between the two that scans them.
 #include "fd_elem.h"
@@ -19,7 +19,7 @@ namespace fd {
 constexpr int ROUTE_ROWS = 512;            // rows of a workgroup; two threads a row choose, one places
 constexpr int ROUTE_COLS = 32;             // experts staged at a time
 constexpr int ROUTE_WORDS = ROUTE_ROWS / 64;
-constexpr int ROUTE_SCAN = 512;            // workgroups from which on their counts are scanned
+constexpr int ROUTE_FEW = 16;             // rows of a workgroup with a wave a row
 constexpr int ROUTE_STAGE = ROUTE_ROWS * (ROUTE_COLS + 2);   // rows of 33 words; later 2 words a choice and 2 more of a row
 
 struct RouteArgs {
@@ -27,7 +27,8 @@ struct RouteArgs {
     const uint8_t* mask;
     int rows, experts, k, normalize, blocks;
     float* weights;
-    int32_t *chosen, *slots, *offsets, *source, *counts;     // counts [blocks, experts], scanned [blocks + 1, experts]: the workspace
+    int32_t *chosen, *slots, *offsets, *source;
+    int32_t* counts;                                         // the workspace: [blocks, experts], scanned [blocks + 1, experts]
 };
 
 // Exclusive scan of `v` over the workgroup's first 512 threads, in `words` (an int of LDS a wave).  `all`: the sum.
@@ -226,99 +227,105 @@ __global__ __launch_bounds__(2 * ROUTE_ROWS) void expert_choose_kernel(RouteArgs
     }
 }
 
-// Largest value of a wave, and its sum, in every lane: shifts within rows of 16, then row 0 to 1 and 2 to 3, then the half.
-__device__ __forceinline__ float wave_max(float v) {
-#define FD_STEP(CTRL, ROWS) \
-    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, ROWS, 0xf, false)))
-    FD_STEP(0x111, 0xf); FD_STEP(0x112, 0xf); FD_STEP(0x114, 0xf); FD_STEP(0x118, 0xf); FD_STEP(0x142, 0xa); FD_STEP(0x143, 0xc);
-#undef FD_STEP
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
-}
-__device__ __forceinline__ float wave_sum(float v) {
-#define FD_STEP(CTRL, ROWS) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false))
-    FD_STEP(0x111, 0xf); FD_STEP(0x112, 0xf); FD_STEP(0x114, 0xf); FD_STEP(0x118, 0xf); FD_STEP(0x142, 0xa); FD_STEP(0x143, 0xc);
+// Largest value of a wave, or its sum, in every lane: shifts within rows of 16 lanes, then row 0 to 1 and 2 to 3, then the half.
+template <bool SUM>
+__device__ __forceinline__ float wave_all(float v) {
+#define FD_STEP(CTRL, ROWS)                                                                                   \
+    {                                                                                                         \
+        const int bits = __float_as_int(v);                                                                   \
+        const float from = __int_as_float(__builtin_amdgcn_update_dpp(SUM ? 0 : bits, bits, CTRL, ROWS, 0xf, false)); \
+        v = SUM ? v + from : fmaxf(v, from);                                                                  \
+    }
+    FD_STEP(0x111, 0xf) FD_STEP(0x112, 0xf) FD_STEP(0x114, 0xf) FD_STEP(0x118, 0xf) FD_STEP(0x142, 0xa) FD_STEP(0x143, 0xc)
 #undef FD_STEP
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
-// Up to FEW_ROWS rows, one workgroup: a wave takes a row, expert 64 i + l in lane l, and finds its choices one by one; the
-// walk of the other kernel would leave most lanes idle through every expert (5 rows of 145 experts, 8 choices: 6 us, the
-// walk 24; 64 rows of 200: 20 and 28 us; 128 rows of 64 experts, 4 choices: 15 and 9 us).
-constexpr int FEW_ROWS = 64;
-
-template <typename T, int VALUES>
-__global__ __launch_bounds__(2 * ROUTE_ROWS) void expert_choose_few_kernel(RouteArgs a) {
-    __shared__ unsigned long long bits[FD_ROUTE_MAX_EXPERTS];          // of an expert: a bit a row
-    __shared__ int best[FEW_ROWS * FD_ROUTE_MAX_K], base[ROUTE_ROWS], words[2 * ROUTE_WORDS];
+// Rows that would not fill the GPU at two threads a row: a wave takes one, experts VALUES * l .. in lane l, and finds its choices
+// one by one, ROUTE_FEW rows a workgroup (10 rows of 8 experts, 2 choices: 4.0 us; 16, 32 and 64 rows a workgroup of 16
+// waves, one after another or side by side, 4096 rows of 64 experts, 4 choices: 8.7, 9.5 and 13.5 us).
+template <typename T, int VALUES, bool MANY>
+__global__ __launch_bounds__(64 * ROUTE_FEW) void expert_choose_few_kernel(RouteArgs a) {
+    __shared__ unsigned bits[FD_ROUTE_MAX_EXPERTS];          // of an expert: a bit a row
+    __shared__ int best[ROUTE_FEW * FD_ROUTE_MAX_K], base[ROUTE_ROWS], words[ROUTE_FEW];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i < a.experts; i += 2 * ROUTE_ROWS) bits[i] = 0;
+    const int row0 = MANY ? blockIdx.x * ROUTE_FEW : 0, rows = min(ROUTE_FEW, a.rows - row0), row = row0 + wave;
+    for (int i = tid; i < a.experts; i += 64 * ROUTE_FEW) bits[i] = 0;
     __syncthreads();
-    for (int row = wave; row < a.rows; row += 2 * ROUTE_WORDS) {
+    if (wave < rows) {
         const bool live = !a.mask || a.mask[row] != 0;
-        float v[VALUES], all = 0.f;
+        const T* p = (const T*)a.logits + (int64_t)row * a.experts;
+        float v[VALUES];
 #pragma unroll
         for (int i = 0; i < VALUES; ++i) {
-            const int x = 64 * i + lane;
-            v[i] = live && x < a.experts ? fmaxf((float)((const T*)a.logits)[(int64_t)row * a.experts + x], -INFINITY) : -INFINITY;
+            const int x = lane * VALUES + i;
+            const float l = fmaxf((float)p[min(x, a.experts - 1)], -INFINITY);       // not a number: the smallest
+            v[i] = live && x < a.experts ? l : -INFINITY;
         }
-        float first = -INFINITY, mine = 0.f, mine_sum = 0.f;        // lane j keeps exp(choice j - choice 0)
-        int mine_at = -1;
+        float first = -INFINITY, top = -INFINITY, sum = 0.f;                 // lane j keeps choice j
+        int chosen = -1;
         for (int j = 0; j < a.k; ++j) {
-            float m = v[0];
+            float mine = v[0];
+            int x = 0;
 #pragma unroll
-            for (int i = 1; i < VALUES; ++i) m = fmaxf(m, v[i]);
-            m = wave_max(m);
-            if (m == -INFINITY) break;
+            for (int i = 1; i < VALUES; ++i) {
+                x = v[i] > mine ? i : x;
+                mine = fmaxf(mine, v[i]);
+            }
+            const float most = wave_all<false>(mine);
+            if (most == -INFINITY) break;
             if (j == 0) {
-                first = m;
+                first = most;
+                if (!a.normalize)
 #pragma unroll
-                for (int i = 0; i < VALUES; ++i) all += v[i] == first ? 1.f : (v[i] > -INFINITY ? exp_fast(v[i] - first) : 0.f);
+                    for (int i = 0; i < VALUES; ++i) sum += v[i] == most ? 1.f : (v[i] > -INFINITY ? exp_fast(v[i] - most) : 0.f);
             }
-            // the lowest expert that has it, which loses it
-            int at = -1;
-#pragma unroll
-            for (int i = 0; i < VALUES; ++i) {
-                const unsigned long long who = __ballot(v[i] == m);
-                if (at < 0 && who) {
-                    at = 64 * i + __ffsll(who) - 1;
-                    if (lane == (at & 63)) v[i] = -INFINITY;
-                }
-            }
-            const float e = m == first ? 1.f : exp_fast(m - first);
-            mine_sum += e;
+            // the lowest expert that has it loses it
+            const int src = __ffsll((unsigned long long)__ballot(mine == most)) - 1;
+            const int who = __builtin_amdgcn_readlane(lane * VALUES + x, src);
             if (lane == j) {
-                mine = e;
-                mine_at = at;
+                top = most;
+                chosen = who;
             }
-            if (lane == 0) atomicOr(&bits[at], 1ull << row);
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) v[i] = lane == src && x == i ? -INFINITY : v[i];
         }
-        const float sum = a.normalize ? mine_sum : wave_sum(all);
+        const float e = chosen < 0 ? 0.f : (top == first ? 1.f : exp_fast(top - first));
+        sum = wave_all<true>(a.normalize ? e : sum);
         if (lane < a.k) {
             const int64_t i = (int64_t)row * a.k + lane;
-            a.weights[i] = mine_at >= 0 ? mine / sum : 0.f;
-            a.chosen[i] = mine_at;
-            best[i] = mine_at;
+            a.weights[i] = chosen >= 0 ? e / sum : 0.f;
+            a.chosen[i] = chosen;
+            best[wave * a.k + lane] = chosen;
+            if (chosen >= 0) atomicOr(&bits[chosen], 1u << wave);
         }
     }
     __syncthreads();
-    const int n = tid < a.experts ? __popcll(bits[tid]) : 0;
-    int all;
-    const int begin = exclusive_scan(n, words, all);
-    if (tid < ROUTE_ROWS) {
-        base[tid] = begin;
-        if (tid < a.experts) a.offsets[tid] = begin;
+    const int n = tid < a.experts ? __popc(bits[tid]) : 0;
+    int all = 0;
+    if (MANY) {
+        if (tid < a.experts) a.counts[(int64_t)blockIdx.x * a.experts + tid] = n;
+    } else {
+        const int begin = exclusive_scan(n, words, all);
+        if (tid < ROUTE_ROWS) {
+            base[tid] = begin;
+            if (tid < a.experts) a.offsets[tid] = begin;
+        }
+        if (tid == 0) a.offsets[a.experts] = all;
+        __syncthreads();
     }
-    if (tid == 0) a.offsets[a.experts] = all;
-    __syncthreads();
-    for (int i = tid; i < a.rows * a.k; i += 2 * ROUTE_ROWS) {
-        const int row = i / a.k, x = best[i];
+    for (int i = tid; i < rows * a.k; i += 64 * ROUTE_FEW) {
+        const int r = i / a.k, x = best[i];
         int at = -1;
         if (x >= 0) {
-            at = base[x] + __popcll(bits[x] & ((1ull << row) - 1));
-            a.source[at] = row;
+            at = __popc(bits[x] & ((1u << r) - 1));
+            if (!MANY) {
+                at += base[x];
+                a.source[at] = r;
+            }
         }
-        a.slots[i] = at;
-        if (i >= all) a.source[i] = -1;
+        a.slots[(int64_t)row0 * a.k + i] = at;                 // several workgroups: the rank, placed below
+        if (!MANY && i >= all) a.source[i] = -1;
     }
 }
 
@@ -353,36 +360,40 @@ __global__ __launch_bounds__(1024) void expert_scan_kernel(RouteArgs a) {
     if (part == PARTS - 1) counts[(int64_t)a.blocks * a.experts] = at;
 }
 
-// Adds to every choice's rank the choices of earlier experts and of earlier workgroups.  Up to ROUTE_SCAN workgroups each sums
-// the counts of all (SUMS).
-template <bool SUMS>
+// Adds to every choice's rank the choices of earlier experts and of earlier workgroups (of PER rows).  SUMS: each workgroup sums the
+// counts of all.
+template <bool SUMS, int PER>
 __global__ __launch_bounds__(ROUTE_ROWS) void expert_place_kernel(RouteArgs a) {
     __shared__ int before[ROUTE_ROWS], words[ROUTE_WORDS];
     const int t = threadIdx.x;
-    // the row's first choices are asked for before the counts, whose sums they wait for
-    const int row = blockIdx.x * ROUTE_ROWS + t;
+    // a thread's first choices are asked for before the counts, whose sums they wait for
+    const int64_t i0 = (int64_t)blockIdx.x * PER * a.k, end = min(i0 + PER * a.k, (int64_t)a.rows * a.k);
     int c4[4], r4[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const bool is = row < a.rows && j < a.k;
-        c4[j] = is ? a.chosen[(int64_t)row * a.k + j] : -1;
-        r4[j] = is ? a.slots[(int64_t)row * a.k + j] : -1;
+        const int64_t i = i0 + t + j * ROUTE_ROWS;
+        c4[j] = i < end ? a.chosen[i] : -1;
+        r4[j] = i < end ? a.slots[i] : -1;
     }
     int b0 = 0, all = 0;
     if (SUMS) {
         // 512 / lanes threads share an expert, each sums every (512 / lanes)-th workgroup
+        constexpr int U = 16;
         __shared__ int total[ROUTE_ROWS];
         int lanes = 1;
         while (lanes < a.experts) lanes *= 2;
         const int e = t & (lanes - 1), part = t / lanes, parts = ROUTE_ROWS / lanes;
-        if (e < a.experts) {
-#pragma unroll 16
-            for (int b = part; b < a.blocks; b += parts) {
-                const int n = a.counts[(int64_t)b * a.experts + e];
-                all += n;
-                if (b < (int)blockIdx.x) b0 += n;
+        if (e < a.experts)
+            for (int b = part; b < a.blocks; b += U * parts) {
+                int n[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) n[u] = a.counts[(int64_t)min(b + u * parts, a.blocks - 1) * a.experts + e];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (b + u * parts < a.blocks) all += n[u];
+                    if (b + u * parts < (int)blockIdx.x) b0 += n[u];
+                }
             }
-        }
         before[t] = b0;
         total[t] = all;
         __syncthreads();
@@ -406,29 +417,50 @@ __global__ __launch_bounds__(ROUTE_ROWS) void expert_place_kernel(RouteArgs a) {
     }
     __syncthreads();
     auto place = [&](int64_t i, int x, int rank) {
-        if (x < 0) return;
-        const int at = before[x] + rank;
-        a.slots[i] = at;
-        a.source[at] = row;
+        if (x >= 0) {
+            const int at = before[x] + rank;
+            a.slots[i] = at;
+            a.source[at] = (int)(i / a.k);
+        }
+        if (i >= routed) a.source[i] = -1;
     };
 #pragma unroll
-    for (int j = 0; j < 4; ++j) place((int64_t)row * a.k + j, c4[j], r4[j]);
-    if (row < a.rows)
-        for (int j = 4; j < a.k; ++j) place((int64_t)row * a.k + j, a.chosen[(int64_t)row * a.k + j], a.slots[(int64_t)row * a.k + j]);
-    const int64_t n = (int64_t)a.rows * a.k, end = (int64_t)(blockIdx.x + 1) * ROUTE_ROWS * a.k;
-    for (int64_t i = (int64_t)blockIdx.x * ROUTE_ROWS * a.k + t; i < (end < n ? end : n); i += ROUTE_ROWS)
-        if (i >= routed) a.source[i] = -1;
+    for (int j = 0; j < 4; ++j)
+        if (i0 + t + j * ROUTE_ROWS < end) place(i0 + t + j * ROUTE_ROWS, c4[j], r4[j]);
+    for (int64_t i = i0 + t + 4 * ROUTE_ROWS; i < end; i += ROUTE_ROWS) place(i, a.chosen[i], a.slots[i]);
+}
+
+// Whether the counts of the workgroups are scanned by a launch of their own, which takes some 4 us, rather than summed by every
+// workgroup of the next (2048 and 4096 rows of 512 experts, 2 choices, 16 rows a workgroup: 13.9 and 15.1 us with the scan, 16.9
+// without it at 2048; 524288 and 1048576 rows of 64, 4 choices: 62 and 112 us, 69 and 147 without).
+static bool route_scans(int64_t blocks, int experts) { return blocks > 1024 || blocks * experts > 16384; }
+
+// Rows of a workgroup, which is also the choice of the kernel: a wave a row where that many rows at two threads each leave most
+// CUs idle and the experts are enough for 64 lanes (4096 rows: of 16 experts, 8 choices, 9.5 us, walk 19.1; of 64, 4 choices,
+// 9.3 and 16.8; of 512, 16 choices, 23 and 169; 16384 rows of 64, 4 choices: 17.1 both; 32768 of 128, 4 choices: 31 and 24).
+// Up to 512 rows the walk is a single launch (256 rows: of 8 experts, 2 choices, 7.8 and 5.5 us; of 32, 8 choices, 8.7 and 14).
+static int route_rows(int64_t rows, int experts) {
+    const int64_t fill = 128 * experts < 32768 ? 128 * experts : 32768;
+    const bool few = rows <= ROUTE_FEW || (experts >= (rows <= ROUTE_ROWS ? 32 : 16) && rows <= (fill > 8192 ? fill : 8192));
+    return few ? ROUTE_FEW : ROUTE_ROWS;
 }
 
 template <typename T>
-static void launch_choose(const RouteArgs& a, hipStream_t s) {
-    if (a.rows <= FEW_ROWS) {
-        if (a.experts <= 64) hipLaunchKernelGGL((expert_choose_few_kernel<T, 1>), dim3(1), dim3(2 * ROUTE_ROWS), 0, s, a);
-        else if (a.experts <= 256) hipLaunchKernelGGL((expert_choose_few_kernel<T, 4>), dim3(1), dim3(2 * ROUTE_ROWS), 0, s, a);
-        else hipLaunchKernelGGL((expert_choose_few_kernel<T, 8>), dim3(1), dim3(2 * ROUTE_ROWS), 0, s, a);
+static void launch_choose(const RouteArgs& a, bool few, hipStream_t s) {
+    const dim3 grid(a.blocks), block(2 * ROUTE_ROWS);
+    if (few) {
+        const dim3 threads(64 * ROUTE_FEW);
+#define FD_FEW(VALUES)                                                                                                 \
+    do {                                                                                                               \
+        if (a.blocks == 1) hipLaunchKernelGGL((expert_choose_few_kernel<T, VALUES, false>), grid, threads, 0, s, a);   \
+        else hipLaunchKernelGGL((expert_choose_few_kernel<T, VALUES, true>), grid, threads, 0, s, a);                  \
+    } while (0)
+        if (a.experts <= 64) FD_FEW(1);
+        else if (a.experts <= 256) FD_FEW(4);
+        else FD_FEW(8);
+#undef FD_FEW
         return;
     }
-    const dim3 grid(a.blocks), block(2 * ROUTE_ROWS);
     const size_t lds = (size_t)a.experts * ROUTE_WORDS * sizeof(unsigned long long);
 #define FD_CHOOSE(KM, WHOLE) hipLaunchKernelGGL((expert_choose_kernel<T, KM, WHOLE>), grid, block, lds, s, a)
     if (a.experts < 8) {
@@ -442,13 +474,25 @@ static void launch_choose(const RouteArgs& a, hipStream_t s) {
 #undef FD_CHOOSE
 }
 
+static void launch_place(const RouteArgs& a, bool few, hipStream_t s) {
+    const dim3 grid(a.blocks), block(ROUTE_ROWS);
+    if (!route_scans(a.blocks, a.experts)) {
+        if (few) hipLaunchKernelGGL((expert_place_kernel<true, ROUTE_FEW>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((expert_place_kernel<true, ROUTE_ROWS>), grid, block, 0, s, a);
+    } else {
+        if (few) hipLaunchKernelGGL((expert_place_kernel<false, ROUTE_FEW>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((expert_place_kernel<false, ROUTE_ROWS>), grid, block, 0, s, a);
+    }
+}
+
 }  // namespace fd
 
 extern "C" {
 
 int64_t fd_expert_route_workspace(int64_t rows, int experts) {
-    const int64_t blocks = (rows + fd::ROUTE_ROWS - 1) / fd::ROUTE_ROWS;
-    return blocks > 1 ? (blocks + (blocks > fd::ROUTE_SCAN)) * experts * (int64_t)sizeof(int32_t) : 0;
+    const int per = fd::route_rows(rows, experts);
+    const int64_t blocks = (rows + per - 1) / per;
+    return blocks > 1 ? (blocks + fd::route_scans(blocks, experts)) * experts * (int64_t)sizeof(int32_t) : 0;
 }
 
 int fd_expert_route(const void* logits, int dtype, int64_t rows, int experts, int k, const uint8_t* mask, int normalize, float* weights,
@@ -466,22 +510,20 @@ int fd_expert_route(const void* logits, int dtype, int64_t rows, int experts, in
                "fd_expert_route: a workspace of %lld bytes is needed", (long long)fd_expert_route_workspace(rows, experts));
     fd::RouteArgs a;
     a.logits = logits; a.mask = mask; a.rows = (int)rows; a.experts = experts; a.k = k; a.normalize = normalize != 0;
-    a.blocks = rows ? fd::ceil_div(rows, fd::ROUTE_ROWS) : 1;
+    const int per = fd::route_rows(rows, experts);
+    a.blocks = rows ? fd::ceil_div(rows, per) : 1;
     a.weights = weights; a.chosen = chosen; a.slots = slots; a.offsets = offsets; a.source = source_rows; a.counts = (int32_t*)workspace;
     fd::ProfScope scope(fd::as_stream(stream), "expert_route", (double)rows * experts * (2 + k),
                         (double)rows * experts * fd::dtype_bytes(dtype) + 16.0 * rows * k);
     return fd::with_dtype(dtype, [&](auto t) {
-        fd::launch_choose<decltype(t)>(a, fd::as_stream(stream));
+        fd::launch_choose<decltype(t)>(a, per == fd::ROUTE_FEW, fd::as_stream(stream));
         FD_LAUNCH_CHECK();
         if (a.blocks > 1) {
-            const dim3 grid(a.blocks), block(fd::ROUTE_ROWS);
-            if (a.blocks <= fd::ROUTE_SCAN) {
-                hipLaunchKernelGGL(fd::expert_place_kernel<true>, grid, block, 0, fd::as_stream(stream), a);
-            } else {
+            if (fd::route_scans(a.blocks, experts)) {
                 hipLaunchKernelGGL(fd::expert_scan_kernel, dim3(fd::ceil_div(experts, 16)), dim3(1024), 0, fd::as_stream(stream), a);
                 FD_LAUNCH_CHECK();
-                hipLaunchKernelGGL(fd::expert_place_kernel<false>, grid, block, 0, fd::as_stream(stream), a);
             }
+            fd::launch_place(a, per == fd::ROUTE_FEW, fd::as_stream(stream));
             FD_LAUNCH_CHECK();
         }
         return FD_OK;

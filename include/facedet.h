@@ -354,7 +354,7 @@ int fd_detector_tensor(fd_detector* det, const char* name, float* out, int64_t c
 
 #define FD_ROUTE_MAX_EXPERTS 512
 #define FD_ROUTE_MAX_K 16
-/* Bytes of device workspace that fd_expert_route needs (0 for up to 512 rows, otherwise 4 * experts for each 512). */
+/* Bytes of device workspace that fd_expert_route needs (0 where one workgroup takes all rows). */
 int64_t fd_expert_route_workspace(int64_t rows, int experts);
 /* logits [rows, experts].  Per row the k largest logits, by descending logit, equal ones by ascending expert; a logit of
  * -inf or NaN is not chosen, a row whose mask byte (mask [rows], may be NULL) is 0 chooses nothing.

@@ -662,6 +662,15 @@ def test_route_of_many_rows(T, E, k, masked):
     assert torch.equal(r.slots.reshape(-1), slots)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,E,k,normalize,masked", [
+    (17, 8, 2, True, False), (300, 31, 4, False, True), (512, 8, 1, True, True), (513, 12, 2, False, False), (400, 15, 8, True, False),
+    (505, 30, 16, False, True), (8200, 17, 5, True, True), (17, 32, 3, True, False), (16, 512, 16, False, False), (8192, 16, 2, False, True),
+    (2500, 257, 4, True, False), (1100, 450, 7, False, True), (300, 1, 1, True, True), (4000, 6, 6, False, False)])
+def test_route_at_the_borders_of_its_kernels(dtype, T, E, k, normalize, masked):
+    test_route(dtype, T, E, k, normalize, masked)
+
+
 @pytest.mark.parametrize("dtype,bits,quiet", [(torch.float32, torch.int32, 0x7f800001), (torch.float16, torch.int16, 0x7c01),
                                               (torch.bfloat16, torch.int16, 0x7f81)])
 @pytest.mark.parametrize("T", [40, 700])
