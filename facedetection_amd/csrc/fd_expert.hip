@@ -127,6 +127,13 @@ __device__ __forceinline__ int opaque(int v) {
     return v;
 }
 
+// Between what a wave's lanes write to LDS and what other lanes of it read there: the accesses of a wave are carried out in their
+// order, which the compiler keeps only between those of one lane.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // The tiles of all groups when every group is cut into tiles of BM slots, one scan over the offsets by every wave: lane l
 // takes the same number of consecutive groups as any other, they start at slot `start` and have `tiles` tiles from
 // `first` on.  Ends are clamped to [0, slots] and never decrease, so any content of `offsets` stays in bounds.  `ends`
@@ -244,7 +251,7 @@ __device__ __forceinline__ void store_tile(const ExpertArgs& a, int e, int m0, i
     constexpr int ROW = NI * 64;                                       // bytes of a row of NI * 16 sums
     constexpr int FIT = BYTES / (16 * ROW), JP = FIT >= MI ? MI : (FIT >= 4 ? 4 : (FIT >= 2 ? 2 : 1));
     constexpr int MASK = NI * 4 - 1 < 15 ? NI * 4 - 1 : 15;
-    static_assert(JP >= 1 && JP * 16 * ROW <= BYTES && (NI & (NI - 1)) == 0, "a wave's piece of LDS holds 16 rows");
+    static_assert(JP >= 1 && JP * 16 * ROW <= BYTES && MI % JP == 0 && (NI & (NI - 1)) == 0, "a wave's piece of LDS holds 16 rows");
     const int lane = opaque(threadIdx.x & 63);
     // pieces of 8 output columns in a row; a lane stays with one of them and takes every (64 / pieces)-th row
     const int pieces = a.gated ? NI : 2 * NI, q = lane & (pieces - 1), shift = __builtin_ctz(pieces);
@@ -265,6 +272,7 @@ __device__ __forceinline__ void store_tile(const ExpertArgs& a, int e, int m0, i
                 const int r = j * 16 + (lane & 15), at = i * 4 + (lane >> 4);
                 *(f32x4_t*)(part + r * ROW + ((at ^ (r & MASK)) * 16)) = acc[i][p * JP + j];
             }
+        wave_fence();
         for (int r = lane >> shift; r < JP * 16; r += 64 >> shift) {
             const int m = m0 + p * JP * 16 + r;
             if (m >= m1 || left <= 0) break;
@@ -293,6 +301,7 @@ __device__ __forceinline__ void store_tile(const ExpertArgs& a, int e, int m0, i
             }
             store8((T*)a.y + (int64_t)m * a.N + n, left, v);
         }
+        wave_fence();
     }
 }
 
@@ -622,12 +631,14 @@ __device__ __forceinline__ void store_wide(const ExpertArgs& a, int e, int m0, i
             const int at = (GATED ? i / 2 : i) * 2 + (quad >> 1);
             *(T4*)(part + r * (PIECES * 16) + ((at ^ (GATED ? (r >> 2) & 3 : r & 7)) * 16) + (quad & 1) * 8) = q;
         }
+        wave_fence();
 #pragma unroll
         for (int h = 0; h < 16 / ROWS; ++h) {
             const int row = row0 + h * ROWS;
             const u32x4_t q = *(const u32x4_t*)(part + row * (PIECES * 16) + ((p ^ (GATED ? (row >> 2) & 3 : row & 7)) * 16));
             if (m0 + j * 16 + row < m1 && n < a.N) __builtin_memcpy(out + (int64_t)(j * 16 + h * ROWS) * a.N, &q, 16);
         }
+        wave_fence();
     }
 }
 

@@ -248,6 +248,15 @@ WIDE = [
     (130560, 1, 1, 264, 2048, "relu", False, True, True, 0.0, 0.01),
     (32000, 2, 4, 320, 1024, "gelu", True, False, True, 2.0, 0.0),
     (65536, 1, 1, 512, 2056, "silu", False, False, False, 0.0, 0.0),
+    # 256 and 192 rows a tile where those fill the last round best
+    (9496, 1, 1, 136, 1328, "relu", False, True, True, 0.0, 0.0),
+    (12228, 1, 1, 200, 600, "silu", True, False, True, 0.0, 0.01),
+    (9828, 1, 2, 264, 680, None, True, True, False, 0.2, 0.0),
+    (9649, 1, 9, 136, 1464, "gelu", False, True, False, 0.1, 0.0),
+    (8444, 1, 1, 136, 480, None, True, True, True, 0.0, 0.0),
+    (10660, 1, 1, 136, 840, "gelu", False, False, True, 0.0, 0.0),
+    (8157, 1, 1, 264, 616, "relu", True, True, False, 0.0, 0.0),
+    (14530, 1, 9, 136, 576, "silu", False, True, True, 0.1, 0.0),
 ]
 
 
@@ -747,7 +756,9 @@ def test_expert_linear_beyond_31_bits(K, N, S, gather, per):
     (4000, 2, 32, 1024, 1024, "silu", True, False, True, 0.5, 0.0), (600, 2, 16, 512, 512, "gelu", False, False, False, 0.5, 0.1),
     (398, 2, 50, 416, 1003, "relu", False, True, True, 0.5, 0.0), (64, 1, 1, 2048, 256, None, False, True, True, 0.0, 0.0),
     (20, 2, 2, 4104, 100, "silu", True, True, True, 0.0, 0.0), (3000, 1, 4, 1001, 300, None, False, False, True, 0.5, 0.0),
-    (30000, 2, 2, 249, 448, "gelu", False, True, True, 0.5, 0.0), (257, 1, 1, 192, 520, None, True, False, True, 0.0, 0.0),
+    (17532, 1, 20, 72, 136, "silu", True, True, True, 0.1, 0.0), (9838, 1, 20, 72, 131, None, True, False, False, 0.1, 0.0),
+    (13750, 2, 9, 72, 83, "relu", True, True, True, 0.1, 0.02), (30000, 1, 5, 73, 150, "gelu", True, True, True, 0.1, 0.0),
+    (5229, 1, 2, 72, 38, "silu", True, False, True, 0.1, 0.0), (30000, 2, 2, 249, 448, "gelu", False, True, True, 0.5, 0.0), (257, 1, 1, 192, 520, None, True, False, True, 0.0, 0.0),
 ], ids=lambda c: "x".join(str(v) for v in c[:5]))
 def test_expert_linear_other_tiles(dtype, case):
     test_expert_linear(dtype, case)
