@@ -8,7 +8,9 @@
 //
 // Bound by memory: a row is read once, held in registers as float32 through all of this, and written once.  Means and
 // squares are summed in float32 over the registers (two passes, no E[v^2] - mean^2), so the only rounding to the
-// tensors' type is the one at the store; u is computed from the unrounded x'.
+// tensors' type is the one at the store; u is computed from the unrounded x'.  Measured: x float32 and h bfloat16, gate,
+// both norms, 8160 x 1024: 25 us for 100 MB; two choices a row, bfloat16, 6000 x 2048: 31 us for 123 MB, where a large copy
+// takes 21 and 26; the sum alone, 130560 x 1024 with two choices: 134 us for 0.8 GB.
 #include "fd_elem.h"
 
 namespace fd {
