@@ -68,4 +68,18 @@ __device__ __forceinline__ float exp_fast(float d) {
     return e > 0.f && e < INFINITY ? fmaf(e, lost * 0.693147180559945309f, e) : e;      // at the ends `lost` is no number
 }
 
+// Inclusive scan over a wave, of sums or of the largest value (of values from 0 on): shifts within rows of 16 lanes, then the
+// last of row 0 to row 1 and of 2 to 3, then of the half.  Through registers: the six steps by __shfl_up go through LDS, 0.3 us.
+template <bool MAX>
+__device__ __forceinline__ int wave_scan(int v) {
+#define FD_STEP(CTRL, ROWS)                                                             \
+    {                                                                                   \
+        const int from = __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);     \
+        v = MAX ? max(v, from) : v + from;                                              \
+    }
+    FD_STEP(0x111, 0xf) FD_STEP(0x112, 0xf) FD_STEP(0x114, 0xf) FD_STEP(0x118, 0xf) FD_STEP(0x142, 0xa) FD_STEP(0x143, 0xc)
+#undef FD_STEP
+    return v;
+}
+
 }  // namespace fd

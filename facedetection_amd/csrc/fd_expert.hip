@@ -149,16 +149,10 @@ __device__ __forceinline__ TileScan scan_tiles(const ExpertArgs& a, int bm, int*
         upto = max(upto, min(a.offsets[i + 1], a.slots));
         ends[i] = upto;
     }
-    int sum = upto;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(sum, d, 64);
-        if (lane >= d) sum = max(sum, v);
-    }
+    const int most = wave_scan<true>(upto);
     TileScan t;
-    t.routed = __builtin_amdgcn_readlane(sum, 63);
-    t.start = __shfl_up(sum, 1, 64);
-    if (lane == 0) t.start = 0;
+    t.routed = __builtin_amdgcn_readlane(most, 63);
+    t.start = __builtin_amdgcn_update_dpp(0, most, 0x138, 0xf, 0xf, false);       // the lane before's; 0 in the first
     t.tiles = 0;
     int at = t.start;
     for (int i = lane * per; i < min((lane + 1) * per, a.experts); ++i) {
@@ -166,12 +160,7 @@ __device__ __forceinline__ TileScan scan_tiles(const ExpertArgs& a, int bm, int*
         t.tiles += (to - at + bm - 1) / bm;
         at = to;
     }
-    sum = t.tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(sum, d, 64);
-        if (lane >= d) sum += v;
-    }
+    const int sum = wave_scan<false>(t.tiles);
     t.first = sum - t.tiles;
     t.total = __builtin_amdgcn_readlane(sum, 63);
     return t;

@@ -34,12 +34,7 @@ struct RouteArgs {
 // Exclusive scan of `v` over the workgroup's first 512 threads, in `words` (an int of LDS a wave).  `all`: the sum.
 __device__ __forceinline__ int exclusive_scan(int v, int* words, int& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int sum = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int up = __shfl_up(sum, d, 64);
-        if (lane >= d) sum += up;
-    }
+    const int sum = wave_scan<false>(v);
     if (lane == 63) words[wave] = sum;
     __syncthreads();
     int before = 0;
