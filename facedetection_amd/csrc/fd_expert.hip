@@ -296,7 +296,9 @@ __device__ __forceinline__ void store_tile(const ExpertArgs& a, int e, int m0, i
 
 // ---------------------------------------------------------------------------------------------------------------
 // Tile kernel for rows of any length and alignment: BM slots x BN weight rows, 4 waves of (BM/2) x (BN/2), 128 bytes of K a
-// step, operands through registers (D steps ahead, since every load is exposed to the full latency) into two LDS stages.
+// step, operands through registers (D steps ahead) into two LDS stages.  Loads that are not aligned are what bounds it (2331
+// slots, 333 x 1001 float16: 15.2 us, of which 7.5 are the launch, the scan, the row list and the store; 333 x 1024: 10.6).
+// Reading the aligned pieces that cover a row and shifting them on the way to LDS took 17.7, more steps ahead no less.
 // A row of a step is 8 pieces; piece c of row r lies at c ^ ((r >> 1) & 7), which spreads the fragment reads over the banks.
 template <typename T, int BM, int BN, int D, int OCC>
 __global__ __launch_bounds__(256, OCC) void expert_tile_kernel(ExpertArgs a) {
@@ -418,7 +420,8 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void expert_dma_kernel(ExpertArg
         t.n0 = (tile % a.tiles_n) * (a.gated ? BN / 2 : BN);
         if (a.rows && wave < BM / 64) {
             const __amdgpu_buffer_rsrc_t lr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.rows + t.m0), 0, (unsigned)(t.m1 - t.m0) * 4, 0x00020000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(lr, (__attribute__((address_space(3))) void*)(list + wave * 64), 4, (wave * 64 + lane) * 4, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(lr, (__attribute__((address_space(3))) void*)(list + wave * 64), 4,
+                                                     (wave * 64 + lane) * 4, 0, 0, 0);
         }
         return t;
     };
@@ -552,12 +555,12 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void expert_dma_kernel(ExpertArg
 
 // ---------------------------------------------------------------------------------------------------------------
 // Large tiles, 16-bit types: 32 MI x 256 (MI = 8: 256 x 256), one workgroup of 2 x 4 waves a CU.  A wave's 128 x 64 sums fill 128
-// accumulation registers; the
-// products of a 64-byte half step of a CU are 1024 cycles of its matrix units, its fragment reads 768 and the loads into
-// LDS 256 cycles of LDS, so everything that is not a product has to run beside the products: that is what the order below
-// is for.  Measured on 32768 rows x 2048 x 4096: 1.17 PFLOP/s from memory and 1.34 when all rows lie in L2, where the large
-// library product reaches 1.33; in one burst after the barrier the loads cost a tenth of it, a burst of fragment reads
-// another.  Four stages of 64 bytes, which keep three steps on their way, measured slower (1.09): 64-byte requests to L2.
+// accumulation registers; the products of a 64-byte half step of a CU are 1024 cycles of its matrix units, its fragment reads
+// 768 and the loads into LDS 256 cycles of LDS, so everything that is not a product has to run beside the products: that is
+// what the order below is for.  Measured on 32768 rows x 2048 x 4096: 1.22 PFLOP/s from memory and 1.34 when all rows lie in
+// L2, where the large library product reaches 1.33; in one burst after the barrier the loads cost a tenth of it, a burst of
+// fragment reads another.  Four stages of 64 bytes, which keep three steps on their way, measured slower (1.09, against
+// 1.17 of two at that time): 64-byte requests to L2.
 //
 // The products of one row fragment with four weight fragments, sums in accumulation registers.  In assembly because the
 // compiler, with 128 of them and 64 registers of fragments, writes products to other registers than it adds to and spills.
@@ -660,7 +663,8 @@ __global__ __launch_bounds__(512, 2) void expert_wide_kernel(ExpertArgs a, unsig
         t.n0 = (tile % a.tiles_n) * (a.gated ? BN / 2 : BN);
         if (a.rows && wave < ROWS / 64) {
             const __amdgpu_buffer_rsrc_t lr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.rows + t.m0), 0, (unsigned)(t.m1 - t.m0) * 4, 0x00020000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(lr, (__attribute__((address_space(3))) void*)(list + wave * 64), 4, (wave * 64 + opaque(lane)) * 4, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(lr, (__attribute__((address_space(3))) void*)(list + wave * 64), 4,
+                                                     (wave * 64 + opaque(lane)) * 4, 0, 0, 0);
         }
         return t;
     };
@@ -967,11 +971,13 @@ static int launch_expert_stream(ExpertArgs a, hipStream_t stream) {
     return FD_OK;
 }
 
-// rows start on 16-byte borders and their offsets have 31 bits: the operands can be loaded straight into LDS (in two steps of 128 bytes or more)
+// Rows that start on 16-byte borders and whose offsets have 31 bits can be loaded straight into LDS, in two steps of 128
+// bytes or more.
 template <typename T>
 static bool dma_rows(const ExpertArgs& a) {
     const int64_t row = (int64_t)a.K * sizeof(T), limit = int64_t(1) << 31;
-    return a.x_rows > 0 && row % 16 == 0 && row > 128 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0 && a.wrows * row < limit && (a.rows ? a.x_rows : 256) * row < limit;
+    return a.x_rows > 0 && row % 16 == 0 && row > 128 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0 && a.wrows * row < limit &&
+           (a.rows ? a.x_rows : 256) * row < limit;
 }
 
 // Which kernel, by sizes, type and alignment (times in bfloat16 unless said otherwise).
