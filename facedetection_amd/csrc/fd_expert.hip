@@ -984,11 +984,13 @@ static bool dma_rows(const ExpertArgs& a) {
 //
 // The stream kernel for up to 4 rows an expert (20 slots on 8 experts of 2 x 1024 x 2048: 14.9 us, 32 x 64 tiles 16.2 us, 64 x 64
 // 20.6; 512 slots on 64 experts of 2 x 512 x 1024: 34.9, 28.6, 28.3 us), in float32 up to 12 (80 slots on those 8: 39.5,
-// 45, 63 us), and wherever 32 x 64 tiles would leave half of the CUs idle, since it splits K over its waves (20 slots,
-// 2048 x 4096: 11.5 and 25.8 us).  Then with 16 rows at a time up to 32 an expert, beyond with 32 (64 slots, 2048 x 4096: 18.7 and
-// 15.5 us).  Long rows have eight waves a workgroup (float32, the 20 slots: 31.9 us, with four 34.8).
+// 45, 63 us): the weights are the traffic.  Beyond that it is offered beside the tiles, with 16 or 32 rows at a time: it
+// splits K over its waves, so it wins where there are few tiles (200 slots, 256 x 1024: 7.8 us with 16 rows, 10.5 with 32,
+// 18.4 with 32 x 64 tiles; in float16 5.5, 6.6 and 8.3; 500 slots: 11.3, 11.0, 18.6 and 7.3, 6.9, 8.6; 800 slots: 18.0, 16.3,
+// 18.7 and 10.7, 9.5, 8.7).  Its loads bound it, 0.055 us for each of a lane's loads in a step of 128 bytes of K, 0.145 for
+// 16-bit rows off 16-byte borders.  Long rows have eight waves a workgroup (float32, the 20 slots: 31.9 us, with four 34.8).
 //
-// Otherwise tiles.  A CU works through ceil(tiles / CUs) of them, and one step of 128 bytes of K costs a CU (with all CUs busy)
+// Tiles: a CU works through ceil(tiles / CUs) of them, and one step of 128 bytes of K costs a CU (with all CUs busy)
 // 1.75, 1.48 and 1.34 us for 256, 224 and 192 x 256, 0.57 us for 128 x 128, 0.37 us for 64 x 128 and 0.27 us for 64 x 64, but a step
 // of a tile is not shorter than its loads take; the large ones, alone on their CU, need another 3.5 to 4 us for their ends.
 // Large tiles win on many rows an expert (32768 rows, 2048 x 4096: 1.22 PFLOP/s for 256 x 256, 0.93, 0.73 and 0.51 for the small
@@ -1012,10 +1014,10 @@ static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
         const double rows = groups == 1 ? ceil_div(a.slots, bm) : a.slots / (double)bm + groups / 2.0;
         return rows * ceil_div(a.wrows, bn);
     };
-    if (a.slots <= (sizeof(T) == 4 ? 12 : 4) * groups || (a.slots <= 64 * groups && tiles_of(32, 64) < cus / 2)) {
-        if (a.slots > 32 * groups) return launch_expert_stream<T, 2, 4, 4>(a, stream);
-        return row_bytes < 8192 ? launch_expert_stream<T, 1, 4, 4>(a, stream) : launch_expert_stream<T, 1, 8, 4>(a, stream);
-    }
+    const auto stream16 = [](const ExpertArgs& p, hipStream_t q) {
+        return (int64_t)p.K * (int)sizeof(T) < 8192 ? launch_expert_stream<T, 1, 4, 4>(p, q) : launch_expert_stream<T, 1, 8, 4>(p, q);
+    };
+    if (a.slots <= (sizeof(T) == 4 ? 12 : 4) * groups) return stream16(a, stream);
     double least = 0.0;
     Launch best = nullptr;
     // a step costs a CU `step` for each of its tiles but takes `load` at least; `ends`: a tile's start and end
@@ -1027,12 +1029,24 @@ static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
         }
     };
     const bool aligned = dma_rows<T>(a);
+    const bool whole = sizeof(T) == 4 || (((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0 && row_bytes % 16 == 0);
+    auto offer_stream = [&](int mt, Launch launch) {
+        const double step = (whole ? 0.055 : 0.145) * (mt + (a.gated ? 2 : 1)), tiles = tiles_of(16 * mt, a.gated ? 32 : 16) / cus;
+        // of several groups the number of tiles is an estimate, which ceil() would take at its word
+        const double rounds = groups == 1 || tiles <= 1.0 ? ceil(tiles) : 0.5 * (tiles + ceil(tiles)), cost = steps * step * rounds + 0.7 * (mt - 1);
+        if (!best || cost < least) {
+            least = cost;
+            best = launch;
+        }
+    };
+    offer_stream(1, stream16);
+    offer_stream(2, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_stream<T, 2, 4, 4>(p, q); });
     if constexpr (sizeof(T) == 4) {
-        offer(32, 64, 0.30, 0.63, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 32, 64, 2, 4>(p, q); });
+        offer(32, 64, 0.30, 0.45, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 32, 64, 2, 4>(p, q); });
         if (aligned) offer(64, 64, 0.50, 0.90, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 64, 2, 2, 4>(p, q); });
         else offer(64, 64, 0.55, 0.90, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 64, 64, 2, 4>(p, q); });
     } else {
-        offer(32, 64, aligned ? 0.24 : 0.33, 0.36, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 32, 64, 2, 4>(p, q); });
+        offer(32, 64, aligned ? 0.24 : 0.33, aligned ? 0.27 : 0.36, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 32, 64, 2, 4>(p, q); });
         if (!aligned) {
             offer(64, 64, 0.45, 0.45, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 64, 64, 2, 4>(p, q); });
             offer(128, 128, 1.15, 1.15, 1.0, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 128, 128, 1, 2>(p, q); });

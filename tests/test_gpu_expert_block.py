@@ -758,7 +758,9 @@ def test_expert_linear_beyond_31_bits(K, N, S, gather, per):
     (20, 2, 2, 4104, 100, "silu", True, True, True, 0.0, 0.0), (3000, 1, 4, 1001, 300, None, False, False, True, 0.5, 0.0),
     (17532, 1, 20, 72, 136, "silu", True, True, True, 0.1, 0.0), (9838, 1, 20, 72, 131, None, True, False, False, 0.1, 0.0),
     (13750, 2, 9, 72, 83, "relu", True, True, True, 0.1, 0.02), (30000, 1, 5, 73, 150, "gelu", True, True, True, 0.1, 0.0),
-    (5229, 1, 2, 72, 38, "silu", True, False, True, 0.1, 0.0), (30000, 2, 2, 249, 448, "gelu", False, True, True, 0.5, 0.0), (257, 1, 1, 192, 520, None, True, False, True, 0.0, 0.0),
+    (5229, 1, 2, 72, 38, "silu", True, False, True, 0.1, 0.0), (200, 1, 1, 1024, 256, "silu", False, True, True, 0.0, 0.0),
+    (500, 1, 1, 2048, 256, "gelu", True, True, False, 0.0, 0.01), (158, 2, 2, 1215, 768, "silu", False, False, True, 1.0, 0.2),
+    (100, 1, 1, 4104, 40, None, True, False, True, 0.0, 0.0), (333, 3, 4, 515, 77, "relu", True, True, True, 0.5, 0.1), (30000, 2, 2, 249, 448, "gelu", False, True, True, 0.5, 0.0), (257, 1, 1, 192, 520, None, True, False, True, 0.0, 0.0),
 ], ids=lambda c: "x".join(str(v) for v in c[:5]))
 def test_expert_linear_other_tiles(dtype, case):
     test_expert_linear(dtype, case)
