@@ -257,8 +257,10 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const T* y, int64_t
                                                              int64_t rows, int k, T* out) {
     const int64_t row = block_index() * blockDim.y + threadIdx.y;
     if (row >= rows) return;
-    for (int col = (blockIdx.y * blockDim.x + threadIdx.x) * P; col < width; col += gridDim.y * blockDim.x * P) {
-        const int at = min(col, width - P);
+    // unsigned: a width is below 2^31 and a stride at most 2^16 * 2^8 * 8, so the column behind the last one still has 32 bits
+    const unsigned columns = width, stride = gridDim.y * blockDim.x * P;
+    for (unsigned col = (blockIdx.y * blockDim.x + threadIdx.x) * P; col < columns; col += stride) {
+        const unsigned at = min(col, columns - P);
         float acc[P];
 #pragma unroll
         for (int i = 0; i < P; ++i) acc[i] = 0.f;

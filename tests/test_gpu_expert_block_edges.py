@@ -1,0 +1,23 @@
+"""The expert-block operators at the ends of what their documentation allows, against float64 or exact results."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_expert_block import TYPES, U, _close, _gen
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("N", [2 ** 31 - 1, 2 ** 31 - 2 ** 27 + 9])
+def test_expert_combine_of_the_widest_rows(N):
+    """Columns up to the last that an int counts: half of a float16 is exact down to 2^-14, one rounding below."""
+    from facedetection_amd import ops
+    y = torch.randn((1, N), generator=_gen(2), device="cuda", dtype=torch.float16)
+    out = ops.expert_combine(y, torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.full((1, 1), 0.5, device="cuda"))
+    for lo in range(0, N, 2 ** 28):
+        hi = min(N, lo + 2 ** 28)
+        assert torch.equal(out[:, lo:hi], y[:, lo:hi] * 0.5)
+    del out, y
+    torch.cuda.empty_cache()
