@@ -215,10 +215,17 @@ def _row_type(a):
     return t if t in _DTYPES else torch.float32
 
 
+def _int_sizes(name, *sizes):
+    """Sizes that the library takes as an int, which would arrive there as others if they had more bits."""
+    if max(sizes) > 2 ** 31 - 1:
+        raise ValueError("%s: sizes of at most %d, not %s" % (name, 2 ** 31 - 1, sizes))
+
+
 def _rows(a, index, name, dtype=None):
     """A [rows, width] tensor on the GPU in its own type, or in ``dtype`` (another of the three types is refused)."""
     if a.ndim != 2:
         raise ValueError("%s must be [rows, width], not %d-dimensional" % (name, a.ndim))
+    _int_sizes(name, a.shape[1])
     return _typed(a, index, name, dtype)
 
 
@@ -309,8 +316,9 @@ def expert_linear(x, weight, offsets, rows=None, bias=None, activation=None, gat
     T, K = x.shape
     if weight.ndim != 3 or weight.shape[2] != K:
         raise ValueError("weight must be [experts, outputs, %d], not %s" % (K, tuple(weight.shape)))
+    E, n, _ = weight.shape
+    _int_sizes("weight", E, n)
     w = _typed(weight, index, "weight", x.dtype)
-    E, n, _ = w.shape
     if gated and n % 2:
         raise ValueError("a gated weight has two halves of rows, not %d rows" % n)
     N = n // 2 if gated else n
@@ -339,6 +347,7 @@ def _slots_weights(slots, weights, index, rows):
         raise ValueError("slots and weights must both be [rows, k], not %s and %s" % (tuple(slots.shape), tuple(weights.shape)))
     if slots.shape[1] == 0:
         raise ValueError("slots has no columns")
+    _int_sizes("slots", slots.shape[1])
     return _ints(slots, index, "slots"), runtime.rows_to_device(weights, torch.float32, index)
 
 

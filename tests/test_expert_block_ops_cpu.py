@@ -1,0 +1,39 @@
+"""Argument checks of the expert-block operators in ops.py that come before anything is moved to the GPU.  Sizes that a C int
+does not hold would reach the library as other sizes.  No GPU work: the tensors are one element seen many times."""
+import pytest
+import torch
+
+from facedetection_amd import ops, runtime
+
+WIDE = 2 ** 32 + 64          # 64 in an int
+
+
+@pytest.fixture(autouse=True)
+def no_gpu(monkeypatch):
+    monkeypatch.setattr(runtime, "current", lambda: (0, 0))
+    monkeypatch.setattr(runtime, "rows_to_device", lambda array, dtype, index: array)
+
+
+def _seen(*shape, dtype=torch.float16):
+    return torch.zeros((), dtype=dtype).expand(shape)
+
+
+@pytest.mark.parametrize("width", [2 ** 31, WIDE])
+def test_widths_beyond_an_int_are_refused(width):
+    x, one, sl, wt = _seen(1, width), _seen(width, dtype=torch.float32), _seen(1, 2, dtype=torch.int32), _seen(1, 2, dtype=torch.float32)
+    off = _seen(2, dtype=torch.int32)
+    calls = [
+        lambda: ops.expert_route(x, 1),
+        lambda: ops.expert_linear(x, _seen(1, 8, width), off),
+        lambda: ops.expert_linear(_seen(1, 8), _seen(1, width, 8), off),
+        lambda: ops.expert_linear(_seen(1, 8), _seen(width, 1, 8), _seen(width + 1, dtype=torch.int32)),
+        lambda: ops.expert_combine(x, sl, wt),
+        lambda: ops.expert_combine(_seen(1, 8), _seen(1, width, dtype=torch.int32), _seen(1, width, dtype=torch.float32)),
+        lambda: ops.block_norm(x, one),
+        lambda: ops.residual_norm(x, x),
+        lambda: ops.residual_norm(_seen(1, 8), _seen(1, 8), slots=_seen(1, width, dtype=torch.int32), weights=_seen(1, width, dtype=torch.float32)),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError, match="at most 2147483647"):
+            call()
+            pytest.fail("call %d was accepted" % i)
