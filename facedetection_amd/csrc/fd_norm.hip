@@ -296,9 +296,11 @@ int fd_residual_norm(const fd_norm_args* p, void* stream) {
     FD_REQUIRE(p->rows < (int64_t(1) << 31), "fd_residual_norm: too many rows");
     if (p->rows == 0) return FD_OK;
     FD_REQUIRE(p->x, "fd_residual_norm: x is NULL");
-    FD_REQUIRE(p->h ? p->x_out != nullptr : p->pre_weight != nullptr, "fd_residual_norm: no output asked for");
+    // an empty h has no address; with slots it is there all the same, and every slot lies outside of it
+    const void* h = p->h ? p->h : (p->slots && p->h_rows == 0 ? p->x : nullptr);
+    FD_REQUIRE(h ? p->x_out != nullptr : p->pre_weight != nullptr, "fd_residual_norm: no output asked for");
     FD_REQUIRE(!p->pre_weight || p->u, "fd_residual_norm: u is NULL");
-    FD_REQUIRE(p->h || !(p->post_weight || p->gate || p->slots), "fd_residual_norm: post norm, gate and slots belong to h");
+    FD_REQUIRE(h || !(p->post_weight || p->gate || p->slots), "fd_residual_norm: post norm, gate and slots belong to h");
     FD_REQUIRE(!p->post_bias || p->post_weight, "fd_residual_norm: post_bias without post_weight");
     FD_REQUIRE(!p->pre_bias || p->pre_weight, "fd_residual_norm: pre_bias without pre_weight");
     FD_REQUIRE(!p->slots || (p->weights && p->k > 0 && p->h_rows >= 0), "fd_residual_norm: slots need weights and k > 0");
@@ -308,7 +310,7 @@ int fd_residual_norm(const fd_norm_args* p, void* stream) {
     FD_REQUIRE(p->gate_act >= FD_GATE_NONE && p->gate_act <= FD_GATE_TANH, "fd_residual_norm: unknown gate activation");
     FD_REQUIRE(p->eps > 0.f, "fd_residual_norm: eps must be positive");
     fd::NormArgs a;
-    a.x = p->x; a.h = p->h; a.gate = p->gate;
+    a.x = p->x; a.h = h; a.gate = p->gate;
     a.post_weight = p->post_weight; a.post_bias = p->post_bias; a.pre_weight = p->pre_weight; a.pre_bias = p->pre_bias;
     a.weights = p->weights; a.slots = p->slots; a.x_out = p->x_out; a.u = p->u;
     a.rows = p->rows; a.h_rows = p->slots ? p->h_rows : p->rows; a.width = p->width; a.k = p->k;
@@ -317,7 +319,7 @@ int fd_residual_norm(const fd_norm_args* p, void* stream) {
     const double n = (double)p->rows * p->width;
     const int sx = fd::dtype_bytes(p->x_dtype), sh = fd::dtype_bytes(p->h_dtype);
     fd::ProfScope scope(fd::as_stream(stream), "residual_norm", n * 8,
-                        n * (sx + (p->h ? sx + sh * (p->slots ? p->k : 1) : 0) + (p->u ? sh : 0)));
+                        n * (sx + (h ? sx + sh * (p->slots ? p->k : 1) : 0) + (p->u ? sh : 0)));
     return fd::with_dtype(p->h_dtype, [&](auto th) {
         using TH = decltype(th);
         return p->x_dtype == p->h_dtype ? fd::launch_residual_norm<TH, TH>(a, fd::as_stream(stream))

@@ -393,7 +393,7 @@ int fd_expert_combine(const void* y, int dtype, int64_t y_rows, int width, const
  * u = norm(x)                                                 (h == NULL: the norm before a block)
  * norm(v) = v / sqrt(mean(v^2) + eps) * weight + bias, or with layer != 0 of v - mean(v).  post_weight == NULL: h enters
  * without a norm; pre_weight == NULL: u is not computed.  With slots, h is the expert sum of fd_expert_combine over
- * h [h_rows, width].  The gate has gate_rows rows, each for rows / gate_rows consecutive rows of x (1: one for all; the number
+ * h [h_rows, width] (h_rows == 0: h may be NULL, no slot adds anything).  The gate has gate_rows rows, each for rows / gate_rows consecutive rows of x (1: one for all; the number
  * of frames: one per frame; rows: one per row).  x may be float32 beside a 16-bit h; u has h's type.  u is computed from
  * the unrounded x_out.  Outputs do not overlap inputs. */
 typedef struct fd_norm_args {

@@ -21,3 +21,19 @@ def test_expert_combine_of_the_widest_rows(N):
         assert torch.equal(out[:, lo:hi], y[:, lo:hi] * 0.5)
     del out, y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_residual_norm_of_no_expert_rows(dtype):
+    """h has no rows: no slot adds anything, so the norm after the block is that of zeros, its bias."""
+    from facedetection_amd import ops
+    g = _gen(3)
+    x, bias, gate = torch.randn((7, 100), generator=g, device="cuda"), torch.randn((100,), generator=g, device="cuda"), torch.randn((100,), generator=g, device="cuda")
+    slots, weights = torch.arange(14, dtype=torch.int32, device="cuda").reshape(7, 2), torch.ones((7, 2), device="cuda")
+    one = torch.ones(100, device="cuda")
+    empty = torch.empty((0, 100), dtype=dtype, device="cuda")
+    assert torch.equal(ops.residual_norm(x, empty, slots=slots, weights=weights), x)
+    new, u = ops.residual_norm(x, empty, slots=slots, weights=weights, post_weight=one, post_bias=bias, gate=gate, scale=0.5, pre_weight=one)
+    want = x.double() + 0.5 * (gate.double() * bias.double())
+    _close(new, want, 4 * U * (x.double().abs() + want.abs()))
+    assert u.dtype == dtype and torch.equal(u, ops.residual_norm(new, torch.zeros((7, 100), dtype=dtype, device="cuda"), pre_weight=one)[1])
