@@ -420,7 +420,7 @@ def residual_norm(x, h, post_weight=None, post_bias=None, gate=None, gate_activa
         slots, weights = _slots_weights(slots, weights, index, T)
         a.slots, a.weights, a.k = slots.data_ptr(), weights.data_ptr(), slots.shape[1]
     if gate is not None:
-        if gate.ndim not in (1, 2) or gate.shape[-1] != N or (gate.ndim == 2 and (gate.shape[0] == 0 or T % gate.shape[0])):
+        if gate.ndim not in (1, 2) or gate.shape[-1] != N or (gate.ndim == 2 and T and (gate.shape[0] == 0 or T % gate.shape[0])):
             raise ValueError("gate must be [%d] or [G, %d] with G a divisor of %d rows, not %s" % (N, N, T, tuple(gate.shape)))
         gate = runtime.rows_to_device(gate, h.dtype if _row_type(gate) == h.dtype else torch.float32, index)
         a.gate, a.gate_rows = gate.data_ptr(), gate.shape[0] if gate.ndim == 2 else 1

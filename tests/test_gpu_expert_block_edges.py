@@ -37,3 +37,17 @@ def test_residual_norm_of_no_expert_rows(dtype):
     want = x.double() + 0.5 * (gate.double() * bias.double())
     _close(new, want, 4 * U * (x.double().abs() + want.abs()))
     assert u.dtype == dtype and torch.equal(u, ops.residual_norm(new, torch.zeros((7, 100), dtype=dtype, device="cuda"), pre_weight=one)[1])
+
+
+def test_expert_block_of_an_empty_batch():
+    """No rows at all, with a gate row for each of them and with frames of no rows."""
+    from facedetection_amd import ops
+    x, one = torch.empty((0, 24), device="cuda"), torch.ones(24, device="cuda")
+    r = ops.expert_route(torch.empty((0, 3), device="cuda"), 2)
+    u = ops.block_norm(x, one)
+    y = ops.expert_linear(u, torch.ones((3, 24, 24), device="cuda"), r.offsets, rows=r.rows)
+    assert u.shape == y.shape == (0, 24) and ops.expert_combine(y, r.slots, r.weights).shape == (0, 24)
+    for gate in (one, torch.empty((0, 24), device="cuda"), torch.ones((4, 24), device="cuda")):
+        for more in ({}, dict(slots=r.slots, weights=r.weights)):
+            new, u = ops.residual_norm(x, y, gate=gate, gate_activation="sigmoid", post_weight=one, pre_weight=one, **more)
+            assert new.shape == u.shape == (0, 24)
