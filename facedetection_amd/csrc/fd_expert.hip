@@ -100,14 +100,18 @@ __device__ __forceinline__ u32x4_t load_piece(const T* p, int left) {
     return v;
 }
 
+// v * Phi(v).  Phi(v) = erfc(z) / 2 for v < 0 and 1 - erfc(z) / 2 otherwise, z = |v| / sqrt(2).
+// 16-bit results: erfc(z) = exp(-z^2) * (c1 t + .. + c7 t^7), t = 1 / (1 + 0.515 z), whose polynomial is fitted to exp(z^2) erfc(z)
+// over 0 <= z <= 10.5 for the least RELATIVE error, 8.5e-7, by linear programming.  The result is then good in the negative tail
+// too, where it is as small as exp(-z^2): the fit, seven terms and the argument of exp2 are off by less than (48 + 1.5 v^2) * 2^-24
+// of the value, a fortieth of half a step of float16 down to its smallest numbers (v = -5.6) and less of bfloat16 (v = -13).
 template <typename T>
 __device__ __forceinline__ float gelu(float v) {
     if (sizeof(T) == 4) return 0.5f * v * erfcf(-0.70710678118654752f * v);     // no cancellation for v << 0
-    // 16-bit results: Abramowitz and Stegun 7.1.26, erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), t = 1 / (1 + p z), z >= 0, to 1.5e-7
-    const float z = 0.70710678118654752f * fabsf(v), t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * z);
-    const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-    const float half_erfc = 0.5f * poly * __builtin_amdgcn_exp2f(-1.44269504088896341f * z * z);
-    return v * (v < 0.f ? half_erfc : 1.f - half_erfc);
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.36415999f * fabsf(v));       // 0.515 / sqrt(2)
+    const float poly = t * (0.29069942f + t * (0.28760397f + t * (0.27682321f + t * (0.06660392f + t * (0.33762236f + t * (-0.35569667f + t * 0.09634463f))))));
+    const float half = 0.5f * poly, e = __builtin_amdgcn_exp2f(-0.72134752044448170f * v * v);
+    return v < 0.f ? v * half * e : v * (1.f - half * e);
 }
 
 template <typename T>

@@ -51,3 +51,31 @@ def test_expert_block_of_an_empty_batch():
         for more in ({}, dict(slots=r.slots, weights=r.weights)):
             new, u = ops.residual_norm(x, y, gate=gate, gate_activation="sigmoid", post_weight=one, pre_weight=one, **more)
             assert new.shape == u.shape == (0, 24)
+
+
+# S, K, N: the stream kernel, the tiles through registers, the tiles by DMA, the large tiles
+VALUES = [(3, 1, 1), (4000, 1, 1), (4000, 136, 24), (50000, 136, 1024)]
+
+
+def _activated(v, S, K, N, act):
+    """act of the values v, as products: x has one of them a row and zeros, all weights are one."""
+    from facedetection_amd import ops
+    x = torch.zeros((S, K), dtype=v.dtype, device="cuda")
+    x[:, K // 2] = v[:S] if v.numel() >= S else v.repeat(-(-S // v.numel()))[:S]
+    off = torch.tensor([0, S], dtype=torch.int32, device="cuda")
+    y = ops.expert_linear(x, torch.ones((1, N, K), dtype=v.dtype, device="cuda"), off, activation=act)
+    assert torch.equal(y, y[:, :1].expand(S, N))
+    return x[:, K // 2].double(), y[:, 0]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("S,K,N", VALUES)
+def test_gelu_is_good_relative_to_its_value(dtype, S, K, N):
+    """The products are exact.  Of the value's own size: for 16 bits the fitted erfc 15 U, its terms, which cancel by less than
+    half, 24 U, exp2, factors and the rounding before them 8 U, and the argument v^2 / 2, rounded twice with a rounded constant,
+    1.25 v^2 U; for float32 erfcf 32 U, and its argument, rounded once with a rounded constant, 1.3 v^2 U."""
+    v = torch.linspace(-12, 12, 4001, device="cuda").to(dtype)
+    v = torch.cat([torch.tensor([-6.0, -8.0, 2.0], device="cuda").to(dtype), v])
+    v, y = _activated(v, S, K, N, "gelu")
+    want = 0.5 * v * torch.special.erfc(-v * math.sqrt(0.5))
+    _close(y, want, (48 + 1.5 * v * v) * U * want.abs())
