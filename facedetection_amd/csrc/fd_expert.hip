@@ -117,9 +117,15 @@ __device__ __forceinline__ float gelu(float v) {
 template <typename T>
 __device__ __forceinline__ float activate(float v, int act) {
     if (act == FD_ACT_RELU) return v < 0.f ? 0.f : v;         // not a number stays so
-    // hardware exp2 and reciprocal, one unit each: exp(-v) is off by |v| * 2^-24 of itself, v * sigmoid(v) by less than
-    // 2^-24 * (|v| + 1) for every v, below the bound of the sum in front of it
-    if (act == FD_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * v));
+    // 16-bit results: the hardware's exp2 and reciprocal, off by less than (1.5 |v| + 8) * 2^-24 of the value, a hundredth of half a
+    // step; zero from v = -87.3 on, where the value is below 100 * 2^-126 (the form for float32: 1133 against 1110 us for the
+    // gated product of 261120 slots, 64 experts, 1024 -> 2 x 1024 in bfloat16)
+    if (act == FD_ACT_SILU && sizeof(T) == 2) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * v));
+    if (act == FD_ACT_SILU) {
+        // v * e / (1 + e) for v < 0 and v / (1 + e) otherwise, e = exp(-|v|): nothing overflows, at most 12 * 2^-24 of the value
+        const float e = exp_fast(-fabsf(v));
+        return (v < 0.f ? v * e : v) / (1.f + e);
+    }
     if (act == FD_ACT_GELU) return gelu<T>(v);
     return v;
 }

@@ -79,3 +79,16 @@ def test_gelu_is_good_relative_to_its_value(dtype, S, K, N):
     v, y = _activated(v, S, K, N, "gelu")
     want = 0.5 * v * torch.special.erfc(-v * math.sqrt(0.5))
     _close(y, want, (48 + 1.5 * v * v) * U * want.abs())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("S,K,N", VALUES)
+def test_silu_is_good_relative_to_its_value(dtype, S, K, N):
+    """The products are exact.  float32: exp 6 U, 1 + exp, the factor and the quotient 2 U each at most.  16 bits: the argument of
+    exp2, rounded once with a rounded constant, 1.3 |v| U, exp2 and the reciprocal 2 U each, three roundings.  A float32 exp
+    below 2^-126 is zero, and so is the result, below 100 * 2^-126."""
+    v = torch.linspace(-100, 100, 4001, device="cuda").to(dtype)
+    v = torch.cat([torch.tensor([-20.0, -87.5, 8.1], device="cuda").to(dtype), v])
+    v, y = _activated(v, S, K, N, "silu")
+    want = v * torch.sigmoid(v)
+    _close(y, want, (12 if dtype == torch.float32 else 8 + 1.5 * v.abs()) * U * want.abs() + torch.where(v < -87.3, 100 * 2.0 ** -126, 0.0))
