@@ -121,6 +121,7 @@ SIGNATURES = {
     "fd_expert_route": (C.c_int, [vp, C.c_int, C.c_int64, C.c_int, C.c_int, vp, C.c_int, vp, vp, vp, vp, vp, vp, C.c_int64, vp]),
     "fd_expert_linear": (C.c_int, [vp, C.c_int, C.c_int64, C.c_int, vp, C.c_int, C.c_int, vp, vp, C.c_int64, vp, C.c_int, C.c_int,
                                    vp, vp]),
+    "fd_expert_linear_kernel": (C.c_char_p, [vp, C.c_int, C.c_int64, C.c_int, vp, C.c_int, C.c_int, vp, C.c_int64, C.c_int]),
     "fd_expert_combine": (C.c_int, [vp, C.c_int, C.c_int64, C.c_int, vp, vp, C.c_int64, C.c_int, vp, vp]),
     "fd_residual_norm": (C.c_int, [C.POINTER(NormArgs), vp]),
     "fd_detector_tensor": (C.c_int, [vp, C.c_char_p, vp, C.c_int64, C.POINTER(C.c_int64), vp]),

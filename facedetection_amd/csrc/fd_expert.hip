@@ -1014,9 +1014,13 @@ static bool dma_rows(const ExpertArgs& a) {
 // for aligned rows too, 0.24 us a step (796 slots on 50 experts of 1547 x 832: 29.9 us, 64 x 64 33 to 36, 64 x 128 31.3; 320 on
 // 8 experts of 2 x 1024 x 2048: 19.3, 21.0 us).  In float32 the matrix units are slow enough (1/16)
 // that every tile reaches the same rate (126 TFLOP/s) and the smallest wastes the least.
+struct ExpertChoice {
+    int (*launch)(const ExpertArgs&, hipStream_t);
+    const char* name;              // of the kernel and its tile, for fd_expert_linear_kernel
+};
+
 template <typename T>
-static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
-    typedef int (*Launch)(const ExpertArgs&, hipStream_t);
+static ExpertChoice choose_expert(const ExpertArgs& a) {
     const int64_t groups = a.experts < a.slots ? a.experts : a.slots, row_bytes = (int64_t)a.K * sizeof(T);
     const int steps = ceil_div(row_bytes, 128), cus = compute_units();
     auto tiles_of = [&](int bm, int bn) {
@@ -1024,54 +1028,69 @@ static int launch_expert(const ExpertArgs& a, hipStream_t stream) {
         const double rows = groups == 1 ? ceil_div(a.slots, bm) : a.slots / (double)bm + groups / 2.0;
         return rows * ceil_div(a.wrows, bn);
     };
-    const auto stream16 = [](const ExpertArgs& p, hipStream_t q) {
-        return (int64_t)p.K * (int)sizeof(T) < 8192 ? launch_expert_stream<T, 1, 4, 4>(p, q) : launch_expert_stream<T, 1, 8, 4>(p, q);
-    };
-    if (a.slots <= (sizeof(T) == 4 ? 12 : 4) * groups) return stream16(a, stream);
+    const ExpertChoice stream16 = row_bytes < 8192 ? ExpertChoice{[](const ExpertArgs& p, hipStream_t q) { return launch_expert_stream<T, 1, 4, 4>(p, q); }, "stream 16 rows, 4 waves"}
+                                                   : ExpertChoice{[](const ExpertArgs& p, hipStream_t q) { return launch_expert_stream<T, 1, 8, 4>(p, q); }, "stream 16 rows, 8 waves"};
+    if (a.slots <= (sizeof(T) == 4 ? 12 : 4) * groups) return stream16;
     double least = 0.0;
-    Launch best = nullptr;
+    ExpertChoice best = {nullptr, nullptr};
     // a step costs a CU `step` for each of its tiles but takes `load` at least; `ends`: a tile's start and end
-    auto offer = [&](int bm, int bn, double step, double load, double ends, Launch launch) {
+    auto offer = [&](int bm, int bn, double step, double load, double ends, const ExpertChoice& choice) {
         const double rounds = ceil(tiles_of(bm, bn) / cus), cost = steps * fmax(rounds * step, load) + rounds * ends;
-        if (!best || cost < least) {
+        if (!best.launch || cost < least) {
             least = cost;
-            best = launch;
+            best = choice;
         }
     };
     const bool aligned = dma_rows<T>(a);
     const bool whole = sizeof(T) == 4 || (((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0 && row_bytes % 16 == 0);
-    auto offer_stream = [&](int mt, Launch launch) {
+    auto offer_stream = [&](int mt, const ExpertChoice& choice) {
         const double step = (whole ? 0.055 : 0.145) * (mt + (a.gated ? 2 : 1)), tiles = tiles_of(16 * mt, a.gated ? 32 : 16) / cus;
         // of several groups the number of tiles is an estimate, which ceil() would take at its word
         const double rounds = groups == 1 || tiles <= 1.0 ? ceil(tiles) : 0.5 * (tiles + ceil(tiles)), cost = steps * step * rounds + 0.7 * (mt - 1);
-        if (!best || cost < least) {
+        if (!best.launch || cost < least) {
             least = cost;
-            best = launch;
+            best = choice;
         }
     };
     offer_stream(1, stream16);
-    offer_stream(2, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_stream<T, 2, 4, 4>(p, q); });
+    offer_stream(2, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_stream<T, 2, 4, 4>(p, q); }, "stream 32 rows, 4 waves"});
     if constexpr (sizeof(T) == 4) {
-        offer(32, 64, 0.30, 0.45, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 32, 64, 2, 4>(p, q); });
-        if (aligned) offer(64, 64, 0.50, 0.90, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 64, 2, 2, 4>(p, q); });
-        else offer(64, 64, 0.55, 0.90, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 64, 64, 2, 4>(p, q); });
+        offer(32, 64, 0.30, 0.45, 0.3, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 32, 64, 2, 4>(p, q); }, "tile 32 x 64"});
+        if (aligned) offer(64, 64, 0.50, 0.90, 0.3, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 64, 2, 2, 4>(p, q); }, "dma 64 x 64"});
+        else offer(64, 64, 0.55, 0.90, 0.3, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 64, 64, 2, 4>(p, q); }, "tile 64 x 64"});
     } else {
-        offer(32, 64, aligned ? 0.24 : 0.33, aligned ? 0.27 : 0.36, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 32, 64, 2, 4>(p, q); });
+        offer(32, 64, aligned ? 0.24 : 0.33, aligned ? 0.27 : 0.36, 0.3, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 32, 64, 2, 4>(p, q); }, "tile 32 x 64"});
         if (!aligned) {
-            offer(64, 64, 0.45, 0.45, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 64, 64, 2, 4>(p, q); });
-            offer(128, 128, 1.15, 1.15, 1.0, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 128, 128, 1, 2>(p, q); });
+            offer(64, 64, 0.45, 0.45, 0.3, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 64, 64, 2, 4>(p, q); }, "tile 64 x 64"});
+            offer(128, 128, 1.15, 1.15, 1.0, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_tile<T, 128, 128, 1, 2>(p, q); }, "tile 128 x 128"});
         } else {
-            offer(64, 64, 0.27, 0.55, 0.3, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 64, 2, 2, 4>(p, q); });
-            offer(64, 128, 0.37, 0.72, 0.5, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 128, 2, 2, 3>(p, q); });
-            offer(128, 128, 0.57, 0.80, 1.0, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 128, 128, 2, 2, 2>(p, q); });
+            offer(64, 64, 0.27, 0.55, 0.3, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 64, 2, 2, 4>(p, q); }, "dma 64 x 64"});
+            offer(64, 128, 0.37, 0.72, 0.5, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 64, 128, 2, 2, 3>(p, q); }, "dma 64 x 128"});
+            offer(128, 128, 0.57, 0.80, 1.0, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_dma<T, 128, 128, 2, 2, 2>(p, q); }, "dma 128 x 128"});
             if (a.N % 8 == 0 && row_bytes > 256) {
-                offer(192, 256, 1.34, 1.34, 3.4, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 6>(p, q); });
-                offer(224, 256, 1.48, 1.48, 3.6, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 7>(p, q); });
-                offer(256, 256, 1.75, 1.75, 3.9, [](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 8>(p, q); });
+                offer(192, 256, 1.34, 1.34, 3.4, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 6>(p, q); }, "wide 192 x 256"});
+                offer(224, 256, 1.48, 1.48, 3.6, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 7>(p, q); }, "wide 224 x 256"});
+                offer(256, 256, 1.75, 1.75, 3.9, {[](const ExpertArgs& p, hipStream_t q) { return launch_expert_wide<T, 8>(p, q); }, "wide 256 x 256"});
             }
         }
     }
-    return best(a, stream);
+    return best;
+}
+
+// Checks the shape of a call and puts it into `a`, whose pointers and activation are still to be set.
+static int expert_shape(ExpertArgs& a, int dtype, int64_t x_rows, int inner, int experts, int outputs, bool gather, int64_t slots, int gated) {
+    FD_REQUIRE(valid_dtype(dtype), "fd_expert_linear: unknown element type");
+    FD_REQUIRE(x_rows >= 0 && inner > 0 && experts > 0 && outputs > 0 && slots >= 0, "fd_expert_linear: bad shape");
+    FD_REQUIRE(gather || x_rows == slots, "fd_expert_linear: without a row list every row of x is a slot (%lld rows, %lld slots)", (long long)x_rows,
+               (long long)slots);
+    if (slots >= (int64_t(1) << 31) - 1024 || experts > FD_EXPERT_MAX || inner > (1 << 24) || outputs > (1 << 24)) {
+        set_error("fd_expert_linear: at most 2^31 - 1024 slots, %d experts, 2^24 inputs and outputs", FD_EXPERT_MAX);
+        return FD_ERR_LIMIT;
+    }
+    a = ExpertArgs();
+    a.x_rows = x_rows; a.K = inner; a.N = outputs; a.wrows = outputs * (gated ? 2 : 1); a.experts = experts; a.slots = (int)slots;
+    a.gated = gated != 0;
+    return FD_OK;
 }
 
 }  // namespace fd
@@ -1080,25 +1099,27 @@ extern "C" {
 
 int fd_expert_linear(const void* x, int dtype, int64_t x_rows, int inner, const void* weight, int experts, int outputs, const int32_t* offsets,
                      const int32_t* rows, int64_t slots, const void* bias, int activation, int gated, void* y, void* stream) {
-    FD_REQUIRE(fd::valid_dtype(dtype), "fd_expert_linear: unknown element type");
-    FD_REQUIRE(x_rows >= 0 && inner > 0 && experts > 0 && outputs > 0 && slots >= 0, "fd_expert_linear: bad shape");
+    fd::ExpertArgs a;
+    FD_TRY(fd::expert_shape(a, dtype, x_rows, inner, experts, outputs, rows != nullptr, slots, gated));
     FD_REQUIRE(activation >= FD_ACT_NONE && activation <= FD_ACT_GELU, "fd_expert_linear: unknown activation");
-    FD_REQUIRE(rows || x_rows == slots, "fd_expert_linear: without a row list every row of x is a slot (%lld rows, %lld slots)", (long long)x_rows,
-               (long long)slots);
-    if (slots >= (int64_t(1) << 31) - 1024 || experts > FD_EXPERT_MAX || inner > (1 << 24) || outputs > (1 << 24)) {
-        fd::set_error("fd_expert_linear: at most 2^31 - 1024 slots, %d experts, 2^24 inputs and outputs", FD_EXPERT_MAX);
-        return FD_ERR_LIMIT;
-    }
     if (slots == 0) return FD_OK;
     FD_REQUIRE((x || x_rows == 0) && weight && offsets && y, "fd_expert_linear: NULL pointer");
+    a.x = x; a.w = weight; a.bias = bias; a.y = y; a.offsets = offsets; a.rows = rows; a.act = activation;
+    return fd::with_dtype(dtype, [&](auto t) { return fd::choose_expert<decltype(t)>(a).launch(a, fd::as_stream(stream)); });
+}
+
+const char* fd_expert_linear_kernel(const void* x, int dtype, int64_t x_rows, int inner, const void* weight, int experts, int outputs,
+                                    const int32_t* rows, int64_t slots, int gated) {
     fd::ExpertArgs a;
-    a.x = x; a.w = weight; a.bias = bias; a.y = y; a.offsets = offsets; a.rows = rows; a.x_rows = x_rows;
-    a.K = inner; a.N = outputs; a.wrows = outputs * (gated ? 2 : 1); a.experts = experts; a.slots = (int)slots; a.act = activation;
-    a.gated = gated != 0; a.tiles_n = 0;
-    return fd::with_dtype(dtype, [&](auto t) {
-        using T = decltype(t);
-        return fd::launch_expert<T>(a, fd::as_stream(stream));
+    if (fd::expert_shape(a, dtype, x_rows, inner, experts, outputs, rows != nullptr, slots, gated) != FD_OK) return nullptr;
+    if (slots == 0) return "";
+    a.x = x; a.w = weight; a.rows = rows;
+    const char* name = nullptr;
+    fd::with_dtype(dtype, [&](auto t) {
+        name = fd::choose_expert<decltype(t)>(a).name;
+        return FD_OK;
     });
+    return name;
 }
 
 }  // extern "C"

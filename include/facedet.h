@@ -380,6 +380,12 @@ int fd_expert_linear(const void* x, int dtype, int64_t x_rows, int inner, const 
                      const int32_t* offsets, const int32_t* rows, int64_t slots, const void* bias, int activation, int gated,
                      void* y, void* stream);
 
+/* Which kernel and tile fd_expert_linear takes for these arguments on the current device, e.g. "dma 64 x 128": for profiles and
+ * tests.  x, weight and rows are looked at for alignment and NULL only.  "" for no slots; NULL (fd_last_error) for arguments
+ * that it refuses. */
+const char* fd_expert_linear_kernel(const void* x, int dtype, int64_t x_rows, int inner, const void* weight, int experts, int outputs,
+                                    const int32_t* rows, int64_t slots, int gated);
+
 /* out[t] = sum over j of weights[t,j] * y[slots[t,j]], in the order of j; a slot outside [0, y_rows) adds nothing.
  * y [y_rows, width], slots / weights [rows, k], out [rows, width]. */
 int fd_expert_combine(const void* y, int dtype, int64_t y_rows, int width, const int32_t* slots, const float* weights,

@@ -3,7 +3,7 @@ does not hold would reach the library as other sizes.  No GPU work: the tensors 
 import pytest
 import torch
 
-from facedetection_amd import ops, runtime
+from facedetection_amd import _lib, ops, runtime
 
 WIDE = 2 ** 32 + 64          # 64 in an int
 
@@ -37,3 +37,13 @@ def test_widths_beyond_an_int_are_refused(width):
         with pytest.raises(ValueError, match="at most 2147483647"):
             call()
             pytest.fail("call %d was accepted" % i)
+
+
+@pytest.mark.parametrize("change", [dict(dtype=3), dict(inner=0), dict(outputs=0), dict(rows=None, slots=9), dict(experts=1025), dict(slots=(1 << 31) - 1024)])
+def test_expert_linear_kernel_names_a_kernel_for_what_the_operator_takes(change):
+    L = _lib.lib()
+    a = dict(x=4096, dtype=2, x_rows=8, inner=64, weight=4096, experts=4, outputs=8, rows=4096, slots=16, gated=0)
+    assert L.fd_expert_linear_kernel(*a.values()) == b"stream 16 rows, 4 waves"
+    assert L.fd_expert_linear_kernel(*dict(a, slots=0).values()) == b""
+    a.update(change)
+    assert L.fd_expert_linear_kernel(*a.values()) is None and b"fd_expert_linear" in L.fd_last_error()
