@@ -1081,7 +1081,7 @@ static ExpertChoice choose_expert(const ExpertArgs& a) {
 static int expert_shape(ExpertArgs& a, int dtype, int64_t x_rows, int inner, int experts, int outputs, bool gather, int64_t slots, int gated) {
     FD_REQUIRE(valid_dtype(dtype), "fd_expert_linear: unknown element type");
     FD_REQUIRE(x_rows >= 0 && inner > 0 && experts > 0 && outputs > 0 && slots >= 0, "fd_expert_linear: bad shape");
-    FD_REQUIRE(gather || x_rows == slots, "fd_expert_linear: without a row list every row of x is a slot (%lld rows, %lld slots)", (long long)x_rows,
+    FD_REQUIRE(gather || x_rows == slots || slots == 0, "fd_expert_linear: without a row list every row of x is a slot (%lld rows, %lld slots)", (long long)x_rows,
                (long long)slots);
     if (slots >= (int64_t(1) << 31) - 1024 || experts > FD_EXPERT_MAX || inner > (1 << 24) || outputs > (1 << 24)) {
         set_error("fd_expert_linear: at most 2^31 - 1024 slots, %d experts, 2^24 inputs and outputs", FD_EXPERT_MAX);

@@ -371,9 +371,9 @@ int fd_expert_route(const void* logits, int dtype, int64_t rows, int experts, in
 #define FD_ACT_SILU 2
 #define FD_ACT_GELU 3
 #define FD_EXPERT_MAX 1024
-/* Slot s of expert e: y[s] = act(x[r] . weight[e]^T + bias[e]), r = rows[s], or s without a row list (x_rows == slots then).
- * x [x_rows, inner], weight [experts, outputs, inner], bias [experts, outputs] (may be NULL), y [slots, outputs], all of one
- * type.  gated != 0: weight and bias have 2 * outputs rows, and y[s] = act(v[0 .. outputs)) * v[outputs .. 2 * outputs).
+/* Slot s of expert e: y[s] = act(x[r] . weight[e]^T + bias[e]), r = rows[s], or s without a row list (then x_rows == slots, or
+ * there are no slots).  x [x_rows, inner], weight [experts, outputs, inner], bias [experts, outputs] (may be NULL), y [slots,
+ * outputs], all of one type.  gated != 0: weight and bias have 2 * outputs rows, and y[s] = act(v[0 .. outputs)) * v[outputs .. 2 * outputs).
  * offsets [experts + 1] as from fd_expert_route: offsets[0] is taken as 0, values are clamped to [the one before, slots].
  * Slots from offsets[experts] on become zeros; an index of rows outside x reads as a row of zeros. */
 int fd_expert_linear(const void* x, int dtype, int64_t x_rows, int inner, const void* weight, int experts, int outputs,

@@ -47,3 +47,9 @@ def test_expert_linear_kernel_names_a_kernel_for_what_the_operator_takes(change)
     assert L.fd_expert_linear_kernel(*dict(a, slots=0).values()) == b""
     a.update(change)
     assert L.fd_expert_linear_kernel(*a.values()) is None and b"fd_expert_linear" in L.fd_last_error()
+
+
+def test_expert_linear_of_an_empty_row_list():
+    """An empty list has no address; it is no call without a list, whose rows would all be slots."""
+    y = ops.expert_linear(torch.ones((4, 8)), torch.ones((2, 5, 8)), torch.zeros(3, dtype=torch.int32), rows=torch.zeros(0, dtype=torch.int32))
+    assert y.shape == (0, 5)
