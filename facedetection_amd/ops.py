@@ -371,18 +371,24 @@ def _norm_kind(kind):
     return 1 if kind == "layer" else 0
 
 
-def block_norm(x, weight, bias=None, kind="rms", eps=1e-6):
+def block_norm(x, weight, bias=None, kind="rms", eps=1e-6, dtype=None):
     """The norm before a block: x [T, N] -> u [T, N] = x / sqrt(mean(x^2) + eps) * weight + bias, for ``kind="layer"`` of
-    x - mean(x).  weight and bias are float32 [N]."""
+    x - mean(x).  weight and bias are float32 [N].  u has x's type; a float32 x (a residual stream held in float32 beside 16-bit
+    blocks) may give u in the torch type ``dtype``, rounded once, at the end."""
     as_np = not isinstance(x, torch.Tensor)
     index, stream = runtime.current()
     x = _rows(x, index, "x")
     T, N = x.shape
     weight, bias = _params(weight, index, "weight", N), _params(bias, index, "bias", N)
-    u = torch.empty_like(x)
-    t = _DTYPES[x.dtype]
-    a = _lib.NormArgs(x=x.data_ptr(), u=u.data_ptr(), pre_weight=_ptr(weight), pre_bias=_ptr(bias), rows=T, width=N, x_dtype=t, h_dtype=t,
-                      layer=_norm_kind(kind), eps=float(eps))
+    if dtype is None:
+        dtype = x.dtype
+    elif dtype not in _DTYPES or (dtype != x.dtype and x.dtype != torch.float32):
+        raise ValueError("u of %s rows cannot be %s" % (x.dtype, dtype))
+    elif as_np and dtype == torch.bfloat16:
+        raise ValueError("NumPy has no bfloat16")
+    u = torch.empty_like(x, dtype=dtype)
+    a = _lib.NormArgs(x=x.data_ptr(), u=u.data_ptr(), pre_weight=_ptr(weight), pre_bias=_ptr(bias), rows=T, width=N, x_dtype=_DTYPES[x.dtype],
+                      h_dtype=_DTYPES[dtype], layer=_norm_kind(kind), eps=float(eps))
     _lib.check(_lib.lib().fd_residual_norm(C.byref(a), stream))
     return u.cpu().numpy() if as_np else u
 

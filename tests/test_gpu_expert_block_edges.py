@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_expert_block import TYPES, U, _close, _gen
+from test_gpu_expert_block import TYPES, U, _close, _gen, _norm64
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +106,28 @@ def test_gate_is_good_relative_to_its_value(act, width):
     _close(y, want, 12 * U * want.abs() + torch.where((gate < -87.3) & (act == "sigmoid"), 2.0 ** -126, 0.0))
     if act == "sigmoid":
         assert bool((y[gate > -87.3] > 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [1, 7, 250, 400, 1000, 2000, 5000, 16384])
+def test_block_norm_of_a_float32_stream(dtype, width):
+    """u in a 16-bit type from float32 rows, rounded once: the rows have values that 16 bits do not hold."""
+    from facedetection_amd import ops
+    g = _gen(width)
+    for rows, layer in ((3, True), (2100 if width <= 2048 else 5, False)):
+        x = torch.randn((rows, width), generator=g, device="cuda") * 3 + 1000
+        w, b = 1 + 0.3 * torch.randn((width,), generator=g, device="cuda"), torch.randn((width,), generator=g, device="cuda")
+        u = ops.block_norm(x, w, b if layer else None, kind="layer" if layer else "rms", dtype=dtype)
+        assert u.dtype == dtype and u.shape == x.shape
+        _close(u, *_norm64(x.double(), torch.zeros_like(x, dtype=torch.float64), w, b if layer else None, layer))
+
+
+def test_block_norm_refuses_types():
+    from facedetection_amd import ops
+    x, one = torch.zeros((4, 8), device="cuda"), torch.ones(8, device="cuda")
+    assert ops.block_norm(np.ones((4, 8), np.float32), one, dtype=torch.float16).dtype == np.float16
+    for call in (lambda: ops.block_norm(x, one, dtype=torch.float64), lambda: ops.block_norm(x.half(), one, dtype=torch.float32),
+                 lambda: ops.block_norm(x.half(), one, dtype=torch.bfloat16), lambda: ops.block_norm(x, one, dtype="bfloat16"),
+                 lambda: ops.block_norm(np.ones((4, 8), np.float32), one, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError):
+            call()
