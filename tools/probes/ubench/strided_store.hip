@@ -2,7 +2,7 @@
 // float32 tensor (1 KB per row) and adds 1 to it (read + write, like a residual epilogue), either row by row in whole
 // 1 KB rows (mode 0) or as four column chunks of 256 B per row with a pause between the chunks (mode 1: the order of
 // the fused tails' 1x1 chunk loop), or chunked without the pause (mode 2).
-//   hipcc --offload-arch=gfx950 -O3 -o strided_store strided_store.hip && ./strided_store
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o strided_store strided_store.hip && ./strided_store
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef float f32x4 __attribute__((ext_vector_type(4)));
