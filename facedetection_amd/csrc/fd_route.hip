@@ -121,9 +121,19 @@ __global__ __launch_bounds__(2 * ROUTE_ROWS) void expert_choose_kernel(RouteArgs
                 if (sum_at != top[0]) sum = sum_at == -INFINITY ? 0.f : sum * exp_fast(sum_at - top[0]);
                 sum_at = top[0];
                 if (sum_at < INFINITY) {
+                    // exp2 without exp_fast's second term: its relative error grows with the distance that makes the value small.
+                    // Four sums in turn, so that no value goes through more than a few roundings; a distance that is no number or
+                    // too long for anything but zero counts as 200
+                    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll 4
-                    // exp2 without exp_fast's second term: its relative error grows with the distance that makes the value small
-                    for (int c = 0; c < cols; ++c) sum += __builtin_amdgcn_exp2f((fmaxf(mine[c], -INFINITY) - sum_at) * 1.44269504088896341f);
+                    for (int c = 0; c < cols; ++c) {
+                        const float next = s0 + __builtin_amdgcn_exp2f(fmaxf(mine[c] - sum_at, -200.f) * 1.44269504088896341f);
+                        s0 = s1;
+                        s1 = s2;
+                        s2 = s3;
+                        s3 = next;
+                    }
+                    sum += (s0 + s1) + (s2 + s3);
                 } else {
                     for (int c = 0; c < cols; ++c) sum += mine[c] == INFINITY ? 1.f : 0.f;
                 }
