@@ -215,17 +215,17 @@ def _row_type(a):
     return t if t in _DTYPES else torch.float32
 
 
-def _int_sizes(name, *sizes):
-    """Sizes that the library takes as an int, which would arrive there as others if they had more bits."""
-    if max(sizes) > 2 ** 31 - 1:
-        raise ValueError("%s: sizes of at most %d, not %s" % (name, 2 ** 31 - 1, sizes))
+_INT_MAX = 2 ** 31 - 1          # sizes that the library takes as an int would arrive there as others if they had more bits
+
+
+def _too_large(name, size):
+    raise ValueError("%s: sizes of at most %d, not %d" % (name, _INT_MAX, size))
 
 
 def _rows(a, index, name, dtype=None):
     """A [rows, width] tensor on the GPU in its own type, or in ``dtype`` (another of the three types is refused)."""
     if a.ndim != 2:
         raise ValueError("%s must be [rows, width], not %d-dimensional" % (name, a.ndim))
-    _int_sizes(name, a.shape[1])
     return _typed(a, index, name, dtype)
 
 
@@ -283,6 +283,8 @@ def expert_route(logits, top_k, mask=None, normalize=True):
     index, stream = runtime.current()
     x = _rows(logits, index, "logits")
     T, E = x.shape
+    if E > _INT_MAX:
+        _too_large("logits", E)
     k = int(top_k)
     if not 0 < k <= E:
         raise ValueError("top_k must be between 1 and the %d experts, not %d" % (E, k))
@@ -317,7 +319,8 @@ def expert_linear(x, weight, offsets, rows=None, bias=None, activation=None, gat
     if weight.ndim != 3 or weight.shape[2] != K:
         raise ValueError("weight must be [experts, outputs, %d], not %s" % (K, tuple(weight.shape)))
     E, n, _ = weight.shape
-    _int_sizes("weight", E, n)
+    if K > _INT_MAX or E > _INT_MAX or n > _INT_MAX:
+        _too_large("weight", max(K, E, n))
     w = _typed(weight, index, "weight", x.dtype)
     if gated and n % 2:
         raise ValueError("a gated weight has two halves of rows, not %d rows" % n)
@@ -345,9 +348,10 @@ def expert_linear(x, weight, offsets, rows=None, bias=None, activation=None, gat
 def _slots_weights(slots, weights, index, rows):
     if slots.ndim != 2 or tuple(weights.shape) != tuple(slots.shape) or (rows is not None and slots.shape[0] != rows):
         raise ValueError("slots and weights must both be [rows, k], not %s and %s" % (tuple(slots.shape), tuple(weights.shape)))
-    if slots.shape[1] == 0:
+    if not 0 < slots.shape[1] <= _INT_MAX:
+        if slots.shape[1]:
+            _too_large("slots", slots.shape[1])
         raise ValueError("slots has no columns")
-    _int_sizes("slots", slots.shape[1])
     return _ints(slots, index, "slots"), runtime.rows_to_device(weights, torch.float32, index)
 
 
@@ -359,8 +363,11 @@ def expert_combine(y, slots, weights):
     y = _rows(y, index, "y")
     s, w = _slots_weights(slots, weights, index, None)
     T, k = s.shape
-    out = y.new_empty((T, y.shape[1]))
-    _lib.check(_lib.lib().fd_expert_combine(y.data_ptr(), _DTYPES[y.dtype], y.shape[0], y.shape[1], s.data_ptr(), w.data_ptr(), T, k,
+    S, N = y.shape
+    if N > _INT_MAX:
+        _too_large("y", N)
+    out = y.new_empty((T, N))
+    _lib.check(_lib.lib().fd_expert_combine(y.data_ptr(), _DTYPES[y.dtype], S, N, s.data_ptr(), w.data_ptr(), T, k,
                                             out.data_ptr(), stream))
     return out.cpu().numpy() if as_np else out
 
@@ -379,16 +386,18 @@ def block_norm(x, weight, bias=None, kind="rms", eps=1e-6, dtype=None):
     index, stream = runtime.current()
     x = _rows(x, index, "x")
     T, N = x.shape
+    if N > _INT_MAX:
+        _too_large("x", N)
     weight, bias = _params(weight, index, "weight", N), _params(bias, index, "bias", N)
-    if dtype is None:
-        dtype = x.dtype
-    elif dtype not in _DTYPES or (dtype != x.dtype and x.dtype != torch.float32):
+    t = _DTYPES[x.dtype]
+    if dtype is None or dtype is x.dtype:
+        u, th = torch.empty_like(x), t
+    elif dtype not in _DTYPES or t != 0 or (as_np and dtype is torch.bfloat16):          # NumPy has no bfloat16
         raise ValueError("u of %s rows cannot be %s" % (x.dtype, dtype))
-    elif as_np and dtype == torch.bfloat16:
-        raise ValueError("NumPy has no bfloat16")
-    u = torch.empty_like(x, dtype=dtype)
-    a = _lib.NormArgs(x=x.data_ptr(), u=u.data_ptr(), pre_weight=_ptr(weight), pre_bias=_ptr(bias), rows=T, width=N, x_dtype=_DTYPES[x.dtype],
-                      h_dtype=_DTYPES[dtype], layer=_norm_kind(kind), eps=float(eps))
+    else:
+        u, th = torch.empty_like(x, dtype=dtype), _DTYPES[dtype]
+    a = _lib.NormArgs(x=x.data_ptr(), u=u.data_ptr(), pre_weight=_ptr(weight), pre_bias=_ptr(bias), rows=T, width=N, x_dtype=t, h_dtype=th,
+                      layer=_norm_kind(kind), eps=float(eps))
     _lib.check(_lib.lib().fd_residual_norm(C.byref(a), stream))
     return u.cpu().numpy() if as_np else u
 
@@ -410,6 +419,8 @@ def residual_norm(x, h, post_weight=None, post_bias=None, gate=None, gate_activa
     h = _rows(h, index, "h")
     x = _rows(x, index, "x", None if _row_type(x) == torch.float32 else h.dtype)
     T, N = x.shape
+    if N > _INT_MAX:
+        _too_large("x", N)
     if h.shape[1] != N or (slots is None and h.shape[0] != T):
         raise ValueError("h is %s, x is %s" % (tuple(h.shape), tuple(x.shape)))
     if (slots is None) != (weights is None):
