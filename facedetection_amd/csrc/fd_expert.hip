@@ -307,7 +307,8 @@ __device__ __forceinline__ void store_tile(const ExpertArgs& a, int e, int m0, i
 // ---------------------------------------------------------------------------------------------------------------
 // Tile kernel for rows of any length and alignment: BM slots x BN weight rows, 4 waves of (BM/2) x (BN/2), 128 bytes of K a
 // step, operands through registers (D steps ahead) into two LDS stages.  Loads that are not aligned are what bounds it (2331
-// slots, 333 x 1001 float16: 15.2 us, of which 7.5 are the launch, the scan, the row list and the store; 333 x 1024: 10.6).
+// slots, 333 x 1001 float16: 16.5 us with 64 x 64 tiles, 14.4 with 32 x 64, of which 8.2 and 6.5 are the launch, the scan, the row
+// list, the store and the first two steps; 333 x 1024: 10.8 with both).
 // Reading the aligned pieces that cover a row and shifting them on the way to LDS took 17.7, more steps ahead no less.
 // A row of a step is 8 pieces; piece c of row r lies at c ^ ((r >> 1) & 7), which spreads the fragment reads over the banks.
 template <typename T, int BM, int BN, int D, int OCC>
@@ -990,7 +991,15 @@ static bool dma_rows(const ExpertArgs& a) {
            (a.rows ? a.x_rows : 256) * row < limit;
 }
 
-// Which kernel, by sizes, type and alignment (times in bfloat16 unless said otherwise).
+struct ExpertChoice {
+    int (*launch)(const ExpertArgs&, hipStream_t);
+    const char* name;              // of the kernel and its tile, for fd_expert_linear_kernel
+};
+
+// Which kernel, by sizes, type and alignment (times in bfloat16 unless said otherwise).  What each expert gets is known on the
+// device only, so it goes by the average: 4096 slots on 1024 experts of 1024 x 1024 take 513 us spread evenly, 548 with shares of
+// 1 / e, and 148 when one expert has them all, whose weights the stream kernel then reads once for every 16 rows (as the only
+// expert of a call it takes large tiles, 15 us).
 //
 // The stream kernel for up to 4 rows an expert (20 slots on 8 experts of 2 x 1024 x 2048: 14.9 us, 32 x 64 tiles 16.2 us, 64 x 64
 // 20.6; 512 slots on 64 experts of 2 x 512 x 1024: 34.9, 28.6, 28.3 us), in float32 up to 12 (80 slots on those 8: 39.5,
@@ -1009,16 +1018,11 @@ static bool dma_rows(const ExpertArgs& a) {
 // has few (1200 slots on 16 such experts: 29 us with 256 x 256, 21, 20 and 20 us).  The large ones take outputs in eights
 // and three steps or more.
 // Through registers, for rows that are not aligned, it is 1.15 us for 128 x 128, 0.45 for 64 x 64 and 0.33 for 32 x 64 (62682 slots,
-// 1448 x 1001: 394 and 583 us for the first two; 2331 slots, 333 x 1001: 34, 16.0, 15.2 us; 41076 slots on 33 experts of
-// 2 x 47 x 3191: 122, 146, 184 us).  32 x 64 through registers has the shortest step of a single tile and is offered
-// for aligned rows too, 0.24 us a step (796 slots on 50 experts of 1547 x 832: 29.9 us, 64 x 64 33 to 36, 64 x 128 31.3; 320 on
-// 8 experts of 2 x 1024 x 2048: 19.3, 21.0 us).  In float32 the matrix units are slow enough (1/16)
-// that every tile reaches the same rate (126 TFLOP/s) and the smallest wastes the least.
-struct ExpertChoice {
-    int (*launch)(const ExpertArgs&, hipStream_t);
-    const char* name;              // of the kernel and its tile, for fd_expert_linear_kernel
-};
-
+// 1448 x 1001: 394 and 583 us for the first two; 2331 slots, 333 x 1001: 34, 16.5, 14.4 us, of which these costs,
+// fitted to more steps and tiles, take the second; 41076 slots on 33 experts of 2 x 47 x 3191: 122, 146, 184 us).  32 x 64 through
+// registers has the shortest step of a single tile and is offered for aligned rows too, 0.24 us a step (796 slots on 50 experts
+// of 1547 x 832: 29.9 us, 64 x 64 33 to 36, 64 x 128 31.3; 320 on 8 experts of 2 x 1024 x 2048: 19.3, 21.0 us).  In float32 the
+// matrix units are slow enough (1/16) that every tile reaches the same rate (126 TFLOP/s) and the smallest wastes the least.
 template <typename T>
 static ExpertChoice choose_expert(const ExpertArgs& a) {
     const int64_t groups = a.experts < a.slots ? a.experts : a.slots, row_bytes = (int64_t)a.K * sizeof(T);
@@ -1028,8 +1032,9 @@ static ExpertChoice choose_expert(const ExpertArgs& a) {
         const double rows = groups == 1 ? ceil_div(a.slots, bm) : a.slots / (double)bm + groups / 2.0;
         return rows * ceil_div(a.wrows, bn);
     };
-    const ExpertChoice stream16 = row_bytes < 8192 ? ExpertChoice{[](const ExpertArgs& p, hipStream_t q) { return launch_expert_stream<T, 1, 4, 4>(p, q); }, "stream 16 rows, 4 waves"}
-                                                   : ExpertChoice{[](const ExpertArgs& p, hipStream_t q) { return launch_expert_stream<T, 1, 8, 4>(p, q); }, "stream 16 rows, 8 waves"};
+    const ExpertChoice stream16 =
+        row_bytes < 8192 ? ExpertChoice{[](const ExpertArgs& p, hipStream_t q) { return launch_expert_stream<T, 1, 4, 4>(p, q); }, "stream 16 rows, 4 waves"}
+                         : ExpertChoice{[](const ExpertArgs& p, hipStream_t q) { return launch_expert_stream<T, 1, 8, 4>(p, q); }, "stream 16 rows, 8 waves"};
     if (a.slots <= (sizeof(T) == 4 ? 12 : 4) * groups) return stream16;
     double least = 0.0;
     ExpertChoice best = {nullptr, nullptr};

@@ -6,7 +6,8 @@
 //   slots[t,j]   = position of the choice among all choices sorted by (expert, t);  rows[slots[t,j]] = t
 //
 // Bound by the read of the logits, with the walk close behind it (130560 rows of 64 float32 logits, 4 choices of a softmax
-// over all, with mask: 19 us for 33 MB).  Two threads share a row: each walks its half of every 32 experts through LDS
+// over all, with mask: 23.2 us in all for 42 MB; a trace has 18.5 us for this launch and 6.4 for the second).  Two threads share
+// a row: each walks its half of every 32 experts through LDS
 // (staged by coalesced loads, 33 words a row so that the walk has no bank conflicts) and keeps its k best in registers; the
 // first thread then takes the other's in.  Where the rows are too few for that, a wave takes one.  A row's experts are
 // distinct, so the rank of a choice among its workgroup's choices of that expert is a population count over one bit per row:
@@ -247,7 +248,7 @@ __device__ __forceinline__ float wave_all(float v) {
 }
 
 // Rows that would not fill the GPU at two threads a row: a wave takes one, experts VALUES * l .. in lane l, and finds its choices
-// one by one, ROUTE_FEW rows a workgroup (10 rows of 8 experts, 2 choices: 4.0 us; 16, 32 and 64 rows a workgroup of 16
+// one by one, ROUTE_FEW rows a workgroup (10 rows of 8 experts, 2 choices: 2.6 us; 16, 32 and 64 rows a workgroup of 16
 // waves, one after another or side by side, 4096 rows of 64 experts, 4 choices: 8.7, 9.5 and 13.5 us).
 template <typename T, int VALUES, bool MANY>
 __global__ __launch_bounds__(64 * ROUTE_FEW) void expert_choose_few_kernel(RouteArgs a) {
