@@ -141,17 +141,23 @@ constexpr float W4_AT[4][6] = {
 };
 
 // sum_k coef[k] * v[k] over the non-zero coefficients (the table is a compile-time constant: after unrolling
-// only the multiplies that exist remain)
-template <int N>
+// only the multiplies that exist remain).  Of the first two products ROUNDED (0 or 1) is the one that is rounded before it
+// is added, all others are fused: written out, since the compiler may fuse either, and another choice is other last bits.
+template <int ROUNDED, int N>
 __device__ __forceinline__ f32x4 wino_dot(const float (&coef)[N], const f32x4 (&v)[N]) {
+    auto times = [&](int k) { return coef[k] == 1.f ? v[k] : v[k] * coef[k]; };
+    auto add = [&](int k, f32x4 to) {
+        return coef[k] == 1.f ? to + v[k] : __builtin_elementwise_fma(v[k], f32x4{coef[k], coef[k], coef[k], coef[k]}, to);
+    };
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    bool first = true;
+    int terms = 0, first = 0;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         if (coef[k] == 0.f) continue;
-        if (first) acc = coef[k] == 1.f ? v[k] : v[k] * coef[k];
-        else acc += v[k] * coef[k];
-        first = false;
+        if (terms == 0) first = k;
+        else if (terms > 1) acc = add(k, acc);
+        else acc = ROUNDED == 0 ? add(k, times(first)) : add(first, times(k));
+        ++terms;
     }
     return acc;
 }
@@ -180,14 +186,14 @@ __global__ __launch_bounds__(256) void wino4_input_kernel(const float* __restric
                 d[i] = *reinterpret_cast<const f32x4*>(x + (((size_t)b * H + yy) * W + xx) * C + c);
         }
 #pragma unroll
-        for (int i = 0; i < 6; ++i) r[i][j] = wino_dot(W4_BT[i], d);
+        for (int i = 0; i < 6; ++i) r[i][j] = wino_dot<1>(W4_BT[i], d);
     }
     const size_t plane = (size_t)T_pad * C;
     float* o = V + (size_t)t * C + c;
 #pragma unroll
     for (int i = 0; i < 6; ++i)
 #pragma unroll
-        for (int j = 0; j < 6; ++j) *reinterpret_cast<f32x4*>(o + (i * 6 + j) * plane) = wino_dot(W4_BT[j], r[i]);
+        for (int j = 0; j < 6; ++j) *reinterpret_cast<f32x4*>(o + (i * 6 + j) * plane) = wino_dot<1>(W4_BT[j], r[i]);
 }
 
 // one thread: one patch (4x4 outputs), 4 consecutive output channels
@@ -211,7 +217,7 @@ __global__ __launch_bounds__(256) void wino4_output_kernel(const float* __restri
 #pragma unroll
         for (int i = 0; i < 6; ++i) m[i] = *reinterpret_cast<const f32x4*>(p + (i * 6 + j) * plane);
 #pragma unroll
-        for (int a = 0; a < 4; ++a) s[a][j] = wino_dot(W4_AT[a], m);
+        for (int a = 0; a < 4; ++a) s[a][j] = wino_dot<0>(W4_AT[a], m);
     }
     const f32x4 bv = bias ? *reinterpret_cast<const f32x4*>(bias + c) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -222,7 +228,7 @@ __global__ __launch_bounds__(256) void wino4_output_kernel(const float* __restri
         for (int q = 0; q < 4; ++q) {
             const int xx = 4 * tx + q;
             if (xx >= W) continue;
-            f32x4 o = wino_dot(W4_AT[q], s[a]) + bv;
+            f32x4 o = wino_dot<1>(W4_AT[q], s[a]) + bv;
             if (relu) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = fmaxf(o[e], 0.f);
@@ -267,7 +273,7 @@ __global__ __launch_bounds__(256) void wino4_input_split_kernel(const uint8_t* _
             }
         }
 #pragma unroll
-        for (int i = 0; i < 6; ++i) r[i][j] = wino_dot(W4_BT[i], d);
+        for (int i = 0; i < 6; ++i) r[i][j] = wino_dot<1>(W4_BT[i], d);
     }
     const size_t plane = (size_t)T_pad * pitch;
     uint8_t* o = V + (size_t)t * pitch + coff;
@@ -276,7 +282,7 @@ __global__ __launch_bounds__(256) void wino4_input_split_kernel(const uint8_t* _
     for (int i = 0; i < 6; ++i)
 #pragma unroll
         for (int j = 0; j < 6; ++j) {
-            const f32x4 v = wino_dot(W4_BT[j], r[i]);
+            const f32x4 v = wino_dot<1>(W4_BT[j], r[i]);
             f16x4 hi, lo;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -312,7 +318,7 @@ __global__ __launch_bounds__(256) void wino4_output_split_kernel(const float* __
 #pragma unroll
         for (int i = 0; i < 6; ++i) m[i] = *reinterpret_cast<const f32x4*>(p + (i * 6 + j) * plane);
 #pragma unroll
-        for (int a = 0; a < 4; ++a) s[a][j] = wino_dot(W4_AT[a], m);
+        for (int a = 0; a < 4; ++a) s[a][j] = wino_dot<0>(W4_AT[a], m);
     }
     const f32x4 bv = bias ? *reinterpret_cast<const f32x4*>(bias + c) : f32x4{0.f, 0.f, 0.f, 0.f};
     const size_t pitch = (size_t)Cout * 4, coff = split_offset(c);
@@ -325,7 +331,7 @@ __global__ __launch_bounds__(256) void wino4_output_split_kernel(const float* __
         for (int q = 0; q < 4; ++q) {
             const int xx = 4 * tx + q;
             if (xx >= W) continue;
-            const f32x4 o = wino_dot(W4_AT[q], s[a]) + bv;
+            const f32x4 o = wino_dot<1>(W4_AT[q], s[a]) + bv;
             f16x4 hi, lo;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
