@@ -9,6 +9,7 @@ import hashlib
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
@@ -58,7 +59,8 @@ def build(force=False, verbose=True):
     os.makedirs(OBJ, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     headers.append(os.path.join(os.path.dirname(PKG), "include", "facedet.h"))
-    objs, rebuilt = [], False
+    headers.append(os.path.abspath(__file__))          # the flags
+    objs, commands = [], []
     # the id of this source set, as a generated header that only fd_core.hip includes
     bid = source_id()
     id_header = os.path.join(OBJ, "fd_build_id.h")
@@ -76,10 +78,11 @@ def build(force=False, verbose=True):
             cmd = [hipcc] + COMMON + extra + ["-I", OBJ, "-c", s, "-o", o]
             if verbose:
                 print(" ".join(cmd), flush=True)
-            subprocess.check_call(cmd)
-            rebuilt = True
+            commands.append(cmd)
         objs.append(o)
-    if rebuilt or not os.path.exists(LIB):
+    with ThreadPoolExecutor(max_workers=8) as pool:
+        list(pool.map(subprocess.check_call, commands))
+    if commands or not os.path.exists(LIB):
         cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
         if verbose:
             print(" ".join(cmd), flush=True)
